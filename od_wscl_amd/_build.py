@@ -15,8 +15,11 @@ ARCH = "gfx950"
 # -ffp-contract=off: ROI bin / sample coordinates must round exactly like the
 # reference's separate fp32 mul and add (SURVEY.md s7 hard part vii); kernels
 # that want FMAs ask for them explicitly (fmaf / MFMA).
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 -- the compiler forms them from ordinary float code, and some of their
+# forms have given wrong results on this hardware now and then (hipcc's host pass warns that it does not know the feature).
 FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
-         "-fvisibility=hidden", "-Wall", "-Wno-unused-function"]
+         "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 # experiment builds (tools/exp, timing studies that knowingly produce wrong results): ODW_EXTRA_FLAGS="-DODW_EXPERIMENTS"
