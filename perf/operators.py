@@ -13,7 +13,8 @@ its 8-bit output), and the AdamW update of many tensors at once (states in 32 or
             the upper one with the probability of its distance from the lower one; only a v that is not zero never becomes zero
             (at least 2^-16 of its scale, the format's smallest number: a root of zero would make the next update of what the
             rounding left of m).  Random bits: 16 a value from the package's counter-based stream, element counter = position
-            in the concatenation of the tensors.
+            in the concatenation of the tensors; the stream's second key is key[1] + 0x9E3779B9 key[0], so that steps whose
+            keys differ in the first word alone do not draw from one set of numbers.
 
 The scale of a block with largest magnitude a: 2^(floor(log2 a) - k), twice that where a's mantissa is over 1.75 (k = 8 for m, 15 for
 v: the formats' largest values are 1.75 * 2^8 and 1.75 * 2^15); held as its exponent + 127, between 1 and 254.
@@ -257,7 +258,7 @@ def plain_mix(x):
 def plain_bits(first, n, key):
     i = torch.arange(first, first + n, device="cuda")
     h = plain_mix((i & 0xFFFFFFFF) ^ key[0])
-    return plain_mix((h + key[1] + (i >> 32)) & 0xFFFFFFFF)
+    return plain_mix((h + key[1] + 0x9E3779B9 * key[0] + (i >> 32)) & 0xFFFFFFFF)
 
 
 def plain_encode(x, rand, k, bias, mantissa, least):
@@ -440,7 +441,7 @@ def exact_random(first, n, key):
             a, b = w // 65536, w % 65536                        # 32-bit product in two halves
             w = ((a * factor % 65536) * 65536 + b * factor) % (1 << 32)
         return w
-    w = scramble((scramble(torch.bitwise_xor(low, torch.full_like(low, key[0]))) + key[1] + high) % (1 << 32))
+    w = scramble((scramble(torch.bitwise_xor(low, torch.full_like(low, key[0]))) + (key[1] + key[0] * 0x9E3779B9) % (1 << 32) + high) % (1 << 32))
     return (w % 65536 + 0.5).double() / 65536, (w // 65536 + 0.5).double() / 65536
 
 
