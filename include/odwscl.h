@@ -697,6 +697,51 @@ int odw_roi_pool_stack_backward_scaled(const void* dX, int dx_is_f32, int ld, co
 int odw_stream_create_cu_mask(int n_words, const uint32_t* mask, void** stream_out);
 int odw_stream_destroy(void* stream);
 
+/* ---- AdamW over many tensors, gradient norm and clipping ------------------------------------------------
+ * beside odw_sgd_momentum (solver/build.py:10-24 builds SGD only; no reference counterpart).  Lists are HOST arrays of
+ * n_tensors entries holding device pointers; tensors are dense, must not overlap, and may be empty (n = 0).
+ *   types[i]: bit 0 = p is bf16 (else fp32), bit 1 = g is bf16 (else fp32); m, v fp32; copy (nullable list of nullable
+ *   pointers) = a bf16 copy of p written in the same pass; lr, wd per tensor.
+ *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2;  g' = g * grad_mult * *grad_scale (device, nullable)
+ *   p -= lr (m / (1 - beta1^step) / (sqrt(v / (1 - beta2^step)) + eps) + wd p)
+ * eps >= 1e-15.  step: the number of this step, from 1; or (bias != NULL) bias = 4 device floats left by odw_adamw_advance, which adds 1 to a
+ * device step counter: the form a captured launch can replay.  max_workgroups as in odw_sgd_momentum_paced (0 = no limit). */
+int odw_adamw(int n_tensors, void* const* p, const void* const* g, void* const* m, void* const* v, void* const* copy,
+              const int64_t* n, const int* types, const float* lr, const float* wd, double beta1, double beta2, double eps,
+              int64_t step, const float* bias, const float* grad_scale, float grad_mult, int max_workgroups, void* stream);
+/* The same with 8-bit states: m = float8 e4m3 (OCP, no infinity), v = float8 e5m2 codes of n[i] bytes, e[i] = 2 bytes for each 256
+ * elements of the tensor: exponent + 127 of the power-of-two scales of m and v.  Rounded stochastically with 16 bits a value of the
+ * counter-based stream (k0, k1 + 0x9E3779B9 k0); the counter of an element is its position in the concatenation of the list's tensors (with
+ * bias != NULL the step is added to k1).  Non-finite averages become NaN codes. */
+int odw_adamw8(int n_tensors, void* const* p, const void* const* g, void* const* m, void* const* v, uint8_t* const* e,
+               void* const* copy, const int64_t* n, const int* types, const float* lr, const float* wd, double beta1, double beta2,
+               double eps, int64_t step, const float* bias, const float* grad_scale, float grad_mult, uint32_t k0, uint32_t k1,
+               int max_workgroups, void* stream);
+int odw_adamw_advance(int64_t* step, double beta1, double beta2, float* bias, void* stream);
+/* out[0] = sqrt(sum of g^2 over all tensors) (summed in fp64, one order), out[1] = min(1, max_norm / (out[0] + 1e-6)).
+ * types[i] bit 1 = bf16.  max_norm may be infinity. */
+int64_t odw_grad_norm_workspace(int n_tensors, const int64_t* n);
+int odw_grad_norm(int n_tensors, const void* const* g, const int64_t* n, const int* types, double max_norm, float* out,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+/* x *= *scale (device) over all tensors, in place. */
+int odw_scale_tensors(int n_tensors, void* const* x, const int64_t* n, const int* types, const float* scale, void* stream);
+
+/* ---- root-mean-square norm of rows -------------------------------------------------------------------------
+ * beside odw_l2norm_rows (no reference counterpart).  x (R x D, row stride ld_x), res (nullable, row stride ld_res):
+ *   h = round(x + res) (dense; h = x without res), rstd[r] = (mean(h_r^2) + eps)^(-1/2) (nullable), y = h rstd w (dense; w nullable)
+ * types: bit 0 = x, y, dy, dx are bf16, bit 1 = res, h, dh, dres are bf16, bit 2 = w, dw are bf16 (else fp32; without res bit 1
+ * has to equal bit 0).
+ * _fp8: y as e4m3 codes q (dense) with one scale a row, max |y_r| / 448 (at least 2^-126): y ~ q * scale.
+ * _bwd: dx = dres = rstd (w dy - h rstd^2 mean(w dy h)) + dh; dw = sum over rows of dy h rstd, in one order; every output nullable. */
+int odw_rms_norm(const void* x, int64_t ld_x, const void* res, int64_t ld_res, const void* w, int64_t R, int D, float eps, void* y,
+                 void* h, float* rstd, int types, void* stream);
+int odw_rms_norm_fp8(const void* x, int64_t ld_x, const void* res, int64_t ld_res, const void* w, int64_t R, int D, float eps,
+                     void* q, float* scale, void* h, int types, void* stream);
+int64_t odw_rms_norm_bwd_workspace(int64_t R, int D);
+int odw_rms_norm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh, const void* h, int64_t ld_h, const void* w,
+                     const float* rstd, int64_t R, int D, void* dx, void* dres, void* dw, int types, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libodwscl.so")
 _lib = None
 
+c_d = ctypes.c_double
 c_f = ctypes.c_float
 c_i = ctypes.c_int
 c_l = ctypes.c_int64
@@ -185,6 +186,18 @@ SIGNATURES = {
     "odw_gemm_nt_bf16_absmax": (c_i, [c_p, c_i, c_p, c_i, c_i, c_i, c_i, c_p, c_i, c_f, c_p, c_p, c_l, c_p]),
     "odw_roi_pool_stack_backward_scaled": (c_i, [c_p, c_i, c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_i, c_p, c_i, c_i, c_i, c_i, c_i, c_i,
                                                  c_i, c_i, c_p, c_p, c_l, c_p]),
+    # ---- AdamW over many tensors, gradient norm, root-mean-square norm
+    "odw_adamw": (c_i, [c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_d, c_d, c_d, c_l, c_p, c_p, c_f, c_i, c_p]),
+    "odw_adamw8": (c_i, [c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_d, c_d, c_d, c_l, c_p, c_p, c_f, c_u, c_u, c_i,
+                         c_p]),
+    "odw_adamw_advance": (c_i, [c_p, c_d, c_d, c_p, c_p]),
+    "odw_grad_norm_workspace": (c_l, [c_i, c_p]),
+    "odw_grad_norm": (c_i, [c_i, c_p, c_p, c_p, c_d, c_p, c_p, c_l, c_p]),
+    "odw_scale_tensors": (c_i, [c_i, c_p, c_p, c_p, c_p, c_p]),
+    "odw_rms_norm": (c_i, [c_p, c_l, c_p, c_l, c_p, c_l, c_i, c_f, c_p, c_p, c_p, c_i, c_p]),
+    "odw_rms_norm_fp8": (c_i, [c_p, c_l, c_p, c_l, c_p, c_l, c_i, c_f, c_p, c_p, c_p, c_i, c_p]),
+    "odw_rms_norm_bwd_workspace": (c_l, [c_l, c_i]),
+    "odw_rms_norm_bwd": (c_i, [c_p, c_l, c_p, c_l, c_p, c_l, c_p, c_p, c_l, c_i, c_p, c_p, c_p, c_i, c_p, c_l, c_p]),
 }
 
 

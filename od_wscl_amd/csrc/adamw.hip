@@ -1,0 +1,507 @@
+// adamw.hip -- the AdamW update of many tensors in one launch (states in fp32, or in 8-bit floats with block scales), and the
+// global gradient norm it is clipped by.
+//
+// A launch takes up to kMaxTensors tensors: their pointers and sizes travel in the kernel's arguments (no table in device
+// memory to upload, nothing to keep alive for a captured launch).  The tensors are cut into chunks of kChunk elements; a
+// workgroup finds the tensor of its chunk by bisection over the chunks' prefix -- the index is uniform, so this is scalar work.
+#include "odw_common.h"
+#include "odw_rng.h"
+#include <math.h>
+
+namespace {
+
+constexpr int kMaxTensors = 44;          // (88 B each: the arguments stay under 4 KB)
+constexpr int kChunk = 4096;             // elements a workgroup handles at a time; a multiple of kBlock
+constexpr int kBlock = 256;              // elements that share a scale: one wave, four elements a lane
+constexpr int kThreads = 256;
+
+enum { kPBf16 = 1, kGBf16 = 2, kVec = 4 };
+
+struct Tensor {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    uint8_t* e;                          // exponents + 127 of the block scales, (m, v) pairs
+    unsigned short* copy;                // bf16 copy of p, or null
+    int64_t n;
+    uint64_t first;                      // the random counter of element 0
+    float lr, wd;
+    int flags;
+    int chunk0;                          // chunks of the tensors before this one
+};
+
+struct Args {
+    Tensor t[kMaxTensors];
+    int count, chunks;
+    float b1, b2, omb1, omb2, eps, c1, c2, mult;
+    uint32_t k0, k1;
+    const float* scale;                  // device factor of the gradients, or null
+    const float* bias;                   // device bias corrections and step (odw_adamw_advance), or null: c1, c2
+};
+
+struct NormArgs {
+    const void* g[kMaxTensors];
+    int64_t n[kMaxTensors];
+    int chunk0[kMaxTensors];
+    uint8_t flags[kMaxTensors];
+    int count, chunks;
+};
+
+__device__ __forceinline__ float bf2f(unsigned short h) { return __uint_as_float((uint32_t)h << 16); }
+__device__ __forceinline__ unsigned short f2bf(float f) {      // round to nearest even; NaN stays NaN
+    uint32_t u = __float_as_uint(f);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (unsigned short)((u >> 16) | 0x40);
+    return (unsigned short)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+
+// The tensor that chunk c lies in: the last one whose first chunk is not behind c.
+template <class F>
+__device__ __forceinline__ int find_tensor(F chunk0, int count, int c) {
+    int lo = 0, hi = count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (chunk0(mid) <= c) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// Four elements of a wave's 256: consecutive ones (vec: pointers aligned for it) or 64 apart.
+__device__ __forceinline__ int64_t elem(bool vec, int64_t base, int lane, int j) { return vec ? base + 4 * lane + j : base + lane + 64 * j; }
+
+__device__ __forceinline__ void load4(const void* src, bool bf16, bool vec, int64_t base, int lane, int64_t n, float (&x)[4]) {
+    if (vec && base + 4 * lane + 3 < n) {
+        if (bf16) {
+            const ushort4 u = *reinterpret_cast<const ushort4*>((const unsigned short*)src + base + 4 * lane);
+            x[0] = bf2f(u.x); x[1] = bf2f(u.y); x[2] = bf2f(u.z); x[3] = bf2f(u.w);
+        } else {
+            const float4 u = *reinterpret_cast<const float4*>((const float*)src + base + 4 * lane);
+            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t i = elem(vec, base, lane, j);
+        x[j] = i < n ? (bf16 ? bf2f(((const unsigned short*)src)[i]) : ((const float*)src)[i]) : 0.0f;
+    }
+}
+
+__device__ __forceinline__ void store4(void* dst, bool bf16, bool vec, int64_t base, int lane, int64_t n, const float (&x)[4]) {
+    if (vec && base + 4 * lane + 3 < n) {
+        if (bf16) {
+            ushort4 u;
+            u.x = f2bf(x[0]); u.y = f2bf(x[1]); u.z = f2bf(x[2]); u.w = f2bf(x[3]);
+            *reinterpret_cast<ushort4*>((unsigned short*)dst + base + 4 * lane) = u;
+        } else {
+            *reinterpret_cast<float4*>((float*)dst + base + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t i = elem(vec, base, lane, j);
+        if (i < n) {
+            if (bf16) ((unsigned short*)dst)[i] = f2bf(x[j]);
+            else ((float*)dst)[i] = x[j];
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t load4_u8(const uint8_t* src, bool vec, int64_t base, int lane, int64_t n) {
+    if (vec && base + 4 * lane + 3 < n) return *reinterpret_cast<const uint32_t*>(src + base + 4 * lane);
+    uint32_t u = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t i = elem(vec, base, lane, j);
+        if (i < n) u |= (uint32_t)src[i] << (8 * j);
+    }
+    return u;
+}
+
+__device__ __forceinline__ void store4_u8(uint8_t* dst, bool vec, int64_t base, int lane, int64_t n, uint32_t u) {
+    if (vec && base + 4 * lane + 3 < n) {
+        *reinterpret_cast<uint32_t*>(dst + base + 4 * lane) = u;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t i = elem(vec, base, lane, j);
+        if (i < n) dst[i] = (uint8_t)(u >> (8 * j));
+    }
+}
+
+// ---- the 8-bit states ---------------------------------------------------------------------------------------------------------
+// m: sign, 4 exponent bits (bias 7), 3 mantissa bits, largest value 1.75 * 2^8, no infinity, 0x7F = NaN.
+// v: sign, 5 exponent bits (bias 15), 2 mantissa bits, largest value 1.75 * 2^15, 0x7F = NaN (0x7C = infinity is not written).
+// Value = code * 2^(e - 127).  Decay moves v by 0.1 % a step and the formats' steps are 12-25 %: rounded to nearest, v would stay
+// where it is; the codes are rounded stochastically, so that their expectation moves.  The scales are powers of two: then the grid
+// is the same from step to step, a stored value lies on it, and the rounding's variance a step is (relative change) x (grid
+// step) instead of (grid step)^2 / 6 -- summed over v's memory of 1 / (1 - beta2) steps a standard deviation of ~0.15 of sqrt(v), without
+// a bias of v, instead of one larger than v itself.
+// A v that is not zero is held as 2^-16 of its scale at least.  An element whose gradients are far below its block's largest can have
+// its m rounded up to the smallest number, 2^-17 of the block's largest m; over a v held as zero that would be an update of any size
+// -- over 2^-32 of the block's largest v it is at most lr x a few (largest m <= 3.2 sqrt(largest v) for beta = 0.9, 0.999).
+// All of it is integer arithmetic on the fp32 words: the same bits whatever the launch geometry.
+template <int BIAS, int MANT, uint32_t LEAST>
+__device__ __forceinline__ uint32_t encode8(float x, float inv_scale, uint32_t rand16, bool any_bad) {
+    constexpr int kDrop = 23 - MANT;
+    const float y = fabsf(x) * inv_scale;
+    const uint32_t u = __float_as_uint(y);
+    // the value in units of 2^-kDrop grid steps: the fp32 word, rebiased, or below the smallest normal number fixed point (cut: the
+    // comparison with the random number is the exact one)
+    const uint32_t word = u < ((uint32_t)(128 - BIAS) << 23) ? (uint32_t)(y * __uint_as_float((uint32_t)(149 + BIAS) << 23))
+                                                             : u - ((uint32_t)(127 - BIAS) << 23);
+    uint32_t code = (word + (rand16 << (kDrop - 16)) + (1u << (kDrop - 17))) >> kDrop;
+    if (code < LEAST && x != 0.0f) code = LEAST;
+    if (any_bad && (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u) code = 0x7Fu;
+    return code | ((__float_as_uint(x) >> 31) << 7);
+}
+
+// The scale of 256 values whose largest finite magnitude has the word `mx`: 2^(exponent - TOP), twice that where the mantissa is
+// over 1.75, which the format's largest value 1.75 * 2^TOP could not hold.
+template <int TOP>
+__device__ __forceinline__ int block_exponent(uint32_t mx) {
+    int e = (int)(mx >> 23) - TOP + ((mx & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return e < 1 ? 1 : e;
+}
+
+__device__ __forceinline__ float decode_m(uint32_t code, float scale) {
+    // sign | 7 bits: the normal numbers by rebiasing, the subnormal ones as the distance from 2^-6
+    const uint32_t a = code & 0x7Fu;
+    const bool low = a < 8u;
+    float x = __uint_as_float(((a + (low ? 8u : 0u)) << 20) + (120u << 23));
+    if (low) x -= 0.015625f;
+    if (a == 0x7Fu) x = __uint_as_float(0x7FC00000u);
+    x *= scale;
+    return (code & 0x80u) ? -x : x;
+}
+
+__device__ __forceinline__ float decode_v(uint32_t code, float scale) {
+    const uint32_t a = code & 0x7Fu;
+    const bool low = a < 4u;
+    float x = __uint_as_float(((a + (low ? 4u : 0u)) << 21) + (112u << 23));
+    if (low) x -= 6.103515625e-05f;
+    if (a >= 0x7Cu) x = __uint_as_float(a == 0x7Cu ? 0x7F800000u : 0x7FC00000u);
+    x *= scale;
+    return (code & 0x80u) ? -x : x;
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const uint32_t o = (uint32_t)__shfl_xor((int)x, off, 64);
+        x = x > o ? x : o;
+    }
+    return x;
+}
+
+// One pass: p, g, m, v in, p, m, v (and p's bf16 copy) out.  The averages are formed with one rounding an operation (no
+// contraction), in the order m b1 + g (1 - b1), v b2 + g g (1 - b2).
+template <bool BITS8>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const Args a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float c1 = a.c1, c2 = a.c2;
+    uint32_t k1 = a.k1;
+    if (a.bias) {
+        c1 = a.bias[0];
+        c2 = a.bias[1];
+        k1 += __float_as_uint(a.bias[2]);        // the step's number: a replayed launch draws new bits
+    }
+    const float gs = a.scale ? a.mult * *a.scale : a.mult;
+    const float rc2 = 1.0f / sqrtf(c2);
+    for (int c = blockIdx.x; c < a.chunks; c += gridDim.x) {
+        const int ti = find_tensor([&](int i) { return a.t[i].chunk0; }, a.count, c);
+        const Tensor& t = a.t[ti];
+        const int64_t n = t.n, c_begin = (int64_t)(c - t.chunk0) * kChunk;
+        const int64_t c_end = c_begin + kChunk < n ? c_begin + kChunk : n;
+        const bool vec = t.flags & kVec, pbf = t.flags & kPBf16, gbf = t.flags & kGBf16;
+        const float step = t.lr / c1, decay = t.lr * t.wd;
+        for (int64_t base = c_begin + wave * kBlock; base < c_end; base += (kThreads / 64) * kBlock) {
+            float p[4], g[4], m[4], v[4];
+            load4(t.p, pbf, vec, base, lane, n, p);
+            load4(t.g, gbf, vec, base, lane, n, g);
+            if (BITS8) {
+                const uint32_t um = load4_u8((const uint8_t*)t.m, vec, base, lane, n);
+                const uint32_t uv = load4_u8((const uint8_t*)t.v, vec, base, lane, n);
+                const uint8_t* e = t.e + 2 * (base / kBlock);
+                const float sm = __uint_as_float((uint32_t)e[0] << 23), sv = __uint_as_float((uint32_t)e[1] << 23);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    m[j] = decode_m(um >> (8 * j), sm);
+                    v[j] = decode_v(uv >> (8 * j), sv);
+                }
+            } else {
+                load4(t.m, false, vec, base, lane, n, m);
+                load4(t.v, false, vec, base, lane, n, v);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float gj = g[j] * gs;
+                m[j] = m[j] * a.b1 + gj * a.omb1;
+                v[j] = v[j] * a.b2 + gj * gj * a.omb2;
+                p[j] -= step * m[j] / (sqrtf(v[j]) * rc2 + a.eps) + decay * p[j];
+            }
+            store4(t.p, pbf, vec, base, lane, n, p);
+            if (t.copy) store4(t.copy, true, vec, base, lane, n, p);
+            if (!BITS8) {
+                store4(t.m, false, vec, base, lane, n, m);
+                store4(t.v, false, vec, base, lane, n, v);
+                continue;
+            }
+            uint32_t mm = 0, mv = 0, bad = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool in = elem(vec, base, lane, j) < n;
+                const uint32_t um = in ? __float_as_uint(m[j]) & 0x7FFFFFFFu : 0u, uv = in ? __float_as_uint(v[j]) & 0x7FFFFFFFu : 0u;
+                if (um < 0x7F800000u) mm = mm > um ? mm : um; else bad = 1;
+                if (uv < 0x7F800000u) mv = mv > uv ? mv : uv; else bad = 1;
+            }
+            mm = wave_max(mm);
+            mv = wave_max(mv);
+            const int em = block_exponent<8>(mm), ev = block_exponent<15>(mv);
+            const float im = __uint_as_float((uint32_t)(254 - em) << 23), iv = __uint_as_float((uint32_t)(254 - ev) << 23);
+            uint32_t qm = 0, qv = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint64_t at = t.first + (uint64_t)elem(vec, base, lane, j);
+                const uint32_t r = odw_mix(odw_mix((uint32_t)at ^ a.k0) + k1 + (uint32_t)(at >> 32));
+                qm |= encode8<7, 3, 0>(m[j], im, r & 0xFFFFu, bad) << (8 * j);
+                qv |= encode8<15, 2, 1>(v[j], iv, r >> 16, bad) << (8 * j);
+            }
+            store4_u8((uint8_t*)t.m, vec, base, lane, n, qm);
+            store4_u8((uint8_t*)t.v, vec, base, lane, n, qv);
+            if (lane == 0) {
+                t.e[2 * (base / kBlock)] = (uint8_t)em;
+                t.e[2 * (base / kBlock) + 1] = (uint8_t)ev;
+            }
+        }
+    }
+}
+
+// step += 1 on the device, and what the update needs of it: the bias corrections and the step's low word.
+__global__ void adamw_advance_kernel(int64_t* step, double b1, double b2, float* bias) {
+    const int64_t t = *step + 1;
+    *step = t;
+    bias[0] = (float)(1.0 - pow(b1, (double)t));
+    bias[1] = (float)(1.0 - pow(b2, (double)t));
+    bias[2] = __uint_as_float((uint32_t)t);
+}
+
+// ---- the global norm ------------------------------------------------------------------------------------------------------------
+// Sum of squares of a chunk: fp32 products exact in fp64, summed in fp64 in a fixed order.
+__global__ __launch_bounds__(kThreads) void sqsum_kernel(const NormArgs a, double* __restrict__ partial) {
+    __shared__ double part[kThreads / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = blockIdx.x;
+    const int ti = find_tensor([&](int i) { return a.chunk0[i]; }, a.count, c);
+    const int64_t n = a.n[ti], c_begin = (int64_t)(c - a.chunk0[ti]) * kChunk;
+    const int64_t c_end = c_begin + kChunk < n ? c_begin + kChunk : n;
+    const bool vec = a.flags[ti] & kVec, bf = a.flags[ti] & kGBf16;
+    double s = 0.0;
+    for (int64_t base = c_begin + wave * kBlock; base < c_end; base += (kThreads / 64) * kBlock) {
+        float g[4];
+        load4(a.g[ti], bf, vec, base, lane, n, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += (double)g[j] * (double)g[j];
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if (lane == 0) part[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[c] = part[0] + part[1] + part[2] + part[3];
+}
+
+// out[0] = sqrt(sum of the partial sums), out[1] = min(1, max_norm / (norm + 1e-6)) (NaN stays NaN).
+__global__ __launch_bounds__(1024) void norm_finish_kernel(const double* __restrict__ partial, int count, double max_norm,
+                                                           float* __restrict__ out) {
+    __shared__ double part[16];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < count; i += 1024) s += partial[i];
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < 16; ++i) t += part[i];
+        const double norm = sqrt(t), c = max_norm / (norm + 1e-6);
+        out[0] = (float)norm;
+        out[1] = c > 1.0 ? 1.0f : (float)c;
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void scale_kernel(const NormArgs a, const float* __restrict__ scale) {
+    const float s = *scale;
+    if (s == 1.0f) return;                       // the product would be what is there
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = blockIdx.x;
+    const int ti = find_tensor([&](int i) { return a.chunk0[i]; }, a.count, c);
+    const int64_t n = a.n[ti], c_begin = (int64_t)(c - a.chunk0[ti]) * kChunk;
+    const int64_t c_end = c_begin + kChunk < n ? c_begin + kChunk : n;
+    const bool vec = a.flags[ti] & kVec, bf = a.flags[ti] & kGBf16;
+    for (int64_t base = c_begin + wave * kBlock; base < c_end; base += (kThreads / 64) * kBlock) {
+        float g[4];
+        load4(a.g[ti], bf, vec, base, lane, n, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) g[j] *= s;
+        store4(const_cast<void*>(a.g[ti]), bf, vec, base, lane, n, g);
+    }
+}
+
+bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+constexpr int64_t kMaxElements = (int64_t)1 << 40;           // of one tensor: its chunks fit an int
+
+// Fills `a` with tensors from `i` on (empty ones left out) until it is full; returns the first one not taken.
+int fill_norm_args(NormArgs& a, int i, int n_tensors, const void* const* g, const int64_t* n, const int* types) {
+    a.count = a.chunks = 0;
+    for (; i < n_tensors && a.count < kMaxTensors; ++i) {
+        if (n[i] == 0) continue;
+        if (a.count && a.chunks + chunks_of(n[i]) > INT32_MAX) break;
+        const bool bf = types[i] & kGBf16;
+        a.g[a.count] = g[i];
+        a.n[a.count] = n[i];
+        a.flags[a.count] = (uint8_t)((bf ? kGBf16 : 0) | (aligned(g[i], bf ? 8 : 16) ? kVec : 0));
+        a.chunk0[a.count] = a.chunks;
+        a.chunks += (int)chunks_of(n[i]);
+        ++a.count;
+    }
+    return i;
+}
+
+int check_list(const char* what, int n_tensors, const void* const* g, const int64_t* n, const int* types) {
+    ODW_REQUIRE(n_tensors >= 0 && (n_tensors == 0 || (g && n && types)), "%s: null list", what);
+    for (int i = 0; i < n_tensors; ++i) {
+        ODW_REQUIRE(n[i] >= 0 && n[i] < kMaxElements, "%s: tensor %d has %lld elements", what, i, (long long)n[i]);
+        ODW_REQUIRE(n[i] == 0 || g[i], "%s: tensor %d: null pointer", what, i);
+        ODW_REQUIRE(types[i] >= 0 && types[i] <= 3, "%s: tensor %d: bad type %d", what, i, types[i]);
+        ODW_REQUIRE(aligned(g[i], types[i] & kGBf16 ? 2 : 4), "%s: tensor %d: pointer not aligned to its elements", what, i);
+    }
+    return ODW_OK;
+}
+
+int adamw(bool bits8, int n_tensors, void* const* p, const void* const* g, void* const* m, void* const* v, uint8_t* const* e,
+          void* const* copy, const int64_t* n, const int* types, const float* lr, const float* wd, double beta1, double beta2,
+          double eps, int64_t step, const float* bias, const float* grad_scale, float grad_mult, uint32_t k0, uint32_t k1,
+          int max_workgroups, hipStream_t stream) {
+    const char* what = bits8 ? "adamw8" : "adamw";
+    const int rc = check_list(what, n_tensors, g, n, types);
+    if (rc != ODW_OK) return rc;
+    ODW_REQUIRE(n_tensors == 0 || (p && m && v && lr && wd && (!bits8 || e)), "%s: null list", what);
+    ODW_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "%s: betas %g, %g not in [0, 1)", what, beta1, beta2);
+    ODW_REQUIRE(eps >= 1e-15, "%s: eps %g is under 1e-15 (squares of gradients underflow before they are small beside it)", what, eps);
+    ODW_REQUIRE(bias || step >= 1, "%s: step %lld is not positive", what, (long long)step);
+    ODW_REQUIRE(max_workgroups >= 0, "%s: max_workgroups %d", what, max_workgroups);
+    for (int i = 0; i < n_tensors; ++i) {
+        if (n[i] == 0) continue;
+        ODW_REQUIRE(p[i] && m[i] && v[i] && (!bits8 || e[i]), "%s: tensor %d: null pointer", what, i);
+        ODW_REQUIRE(aligned(p[i], types[i] & kPBf16 ? 2 : 4) && (!copy || aligned(copy[i], 2)) &&
+                        (bits8 || (aligned(m[i], 4) && aligned(v[i], 4))), "%s: tensor %d: pointer not aligned to its elements", what, i);
+    }
+    Args a;
+    a.b1 = (float)beta1; a.b2 = (float)beta2; a.omb1 = (float)(1.0 - beta1); a.omb2 = (float)(1.0 - beta2);
+    a.eps = (float)eps;
+    a.c1 = bias ? 1.0f : (float)(1.0 - pow(beta1, (double)step));
+    a.c2 = bias ? 1.0f : (float)(1.0 - pow(beta2, (double)step));
+    // keys that differ in k0 alone would permute one set of numbers over the elements (the hash starts from counter ^ k0): a small
+    // tensor would meet the same few thousand numbers step after step, and their excess over the mean would not average out
+    a.mult = grad_mult; a.k0 = k0; a.k1 = k1 + 0x9E3779B9u * k0; a.scale = grad_scale; a.bias = bias;
+    uint64_t first = 0;
+    for (int i = 0; i < n_tensors;) {
+        a.count = a.chunks = 0;
+        for (; i < n_tensors && a.count < kMaxTensors; ++i) {
+            if (n[i] == 0) continue;
+            if (a.count && a.chunks + chunks_of(n[i]) > INT32_MAX) break;
+            Tensor& t = a.t[a.count++];
+            t.p = p[i]; t.g = g[i]; t.m = m[i]; t.v = v[i]; t.e = bits8 ? e[i] : nullptr;
+            t.copy = copy ? (unsigned short*)copy[i] : nullptr;
+            t.n = n[i]; t.first = first; t.lr = lr[i]; t.wd = wd[i];
+            const int sb = bits8 ? 4 : 16;
+            const bool vec = aligned(t.p, types[i] & kPBf16 ? 8 : 16) && aligned(t.g, types[i] & kGBf16 ? 8 : 16) && aligned(t.m, sb) &&
+                             aligned(t.v, sb) && aligned(t.copy, 8);
+            t.flags = types[i] | (vec ? kVec : 0);
+            t.chunk0 = a.chunks;
+            a.chunks += (int)chunks_of(n[i]);
+            first += (uint64_t)n[i];
+        }
+        if (!a.count) break;
+        const int grid = max_workgroups > 0 && max_workgroups < a.chunks ? max_workgroups : a.chunks;
+        if (bits8) adamw_kernel<true><<<grid, kThreads, 0, stream>>>(a);
+        else adamw_kernel<false><<<grid, kThreads, 0, stream>>>(a);
+        ODW_CHECK_LAUNCH("adamw_kernel");
+    }
+    return ODW_OK;
+}
+
+}  // namespace
+
+ODW_EXPORT int64_t odw_grad_norm_workspace(int n_tensors, const int64_t* n) {
+    int64_t chunks = 0;
+    for (int i = 0; i < n_tensors; ++i) chunks += n[i] > 0 ? chunks_of(n[i]) : 0;
+    return chunks * (int64_t)sizeof(double);
+}
+
+ODW_EXPORT int odw_grad_norm(int n_tensors, const void* const* g, const int64_t* n, const int* types, double max_norm, float* out,
+                             void* workspace, int64_t workspace_bytes, void* stream_) {
+    hipStream_t stream = (hipStream_t)stream_;
+    const int rc = check_list("grad_norm", n_tensors, g, n, types);
+    if (rc != ODW_OK) return rc;
+    ODW_REQUIRE(out, "grad_norm: null output");
+    ODW_REQUIRE(max_norm > 0.0, "grad_norm: max_norm %g is not positive", max_norm);
+    const int64_t need = odw_grad_norm_workspace(n_tensors, n);
+    if (need > 0 && (!workspace || workspace_bytes < need)) {
+        odw_set_error("grad_norm: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+        return ODW_EWORKSPACE;
+    }
+    ODW_REQUIRE(aligned(workspace, 8), "grad_norm: workspace must be 8-byte aligned");
+    ODW_REQUIRE(need / (int64_t)sizeof(double) <= INT32_MAX, "grad_norm: too many elements");
+    NormArgs a;
+    int done = 0;
+    for (int i = 0; i < n_tensors;) {
+        i = fill_norm_args(a, i, n_tensors, g, n, types);
+        if (!a.count) break;
+        sqsum_kernel<<<a.chunks, kThreads, 0, stream>>>(a, (double*)workspace + done);
+        ODW_CHECK_LAUNCH("sqsum_kernel");
+        done += a.chunks;
+    }
+    norm_finish_kernel<<<1, 1024, 0, stream>>>((const double*)workspace, done, max_norm, out);
+    ODW_CHECK_LAUNCH("norm_finish_kernel");
+    return ODW_OK;
+}
+
+ODW_EXPORT int odw_scale_tensors(int n_tensors, void* const* x, const int64_t* n, const int* types, const float* scale, void* stream_) {
+    const int rc = check_list("scale_tensors", n_tensors, x, n, types);
+    if (rc != ODW_OK) return rc;
+    ODW_REQUIRE(scale, "scale_tensors: null scale");
+    NormArgs a;
+    for (int i = 0; i < n_tensors;) {
+        i = fill_norm_args(a, i, n_tensors, x, n, types);
+        if (!a.count) break;
+        scale_kernel<<<a.chunks, kThreads, 0, (hipStream_t)stream_>>>(a, scale);
+        ODW_CHECK_LAUNCH("scale_kernel");
+    }
+    return ODW_OK;
+}
+
+ODW_EXPORT int odw_adamw_advance(int64_t* step, double beta1, double beta2, float* bias, void* stream_) {
+    ODW_REQUIRE(step && bias, "adamw_advance: null pointer");
+    adamw_advance_kernel<<<1, 1, 0, (hipStream_t)stream_>>>(step, beta1, beta2, bias);
+    ODW_CHECK_LAUNCH("adamw_advance_kernel");
+    return ODW_OK;
+}
+
+ODW_EXPORT int odw_adamw(int n_tensors, void* const* p, const void* const* g, void* const* m, void* const* v, void* const* copy,
+                         const int64_t* n, const int* types, const float* lr, const float* wd, double beta1, double beta2, double eps,
+                         int64_t step, const float* bias, const float* grad_scale, float grad_mult, int max_workgroups, void* stream_) {
+    return adamw(false, n_tensors, p, g, m, v, nullptr, copy, n, types, lr, wd, beta1, beta2, eps, step, bias, grad_scale, grad_mult, 0,
+                 0, max_workgroups, (hipStream_t)stream_);
+}
+
+ODW_EXPORT int odw_adamw8(int n_tensors, void* const* p, const void* const* g, void* const* m, void* const* v, uint8_t* const* e,
+                          void* const* copy, const int64_t* n, const int* types, const float* lr, const float* wd, double beta1,
+                          double beta2, double eps, int64_t step, const float* bias, const float* grad_scale, float grad_mult,
+                          uint32_t k0, uint32_t k1, int max_workgroups, void* stream_) {
+    return adamw(true, n_tensors, p, g, m, v, e, copy, n, types, lr, wd, beta1, beta2, eps, step, bias, grad_scale, grad_mult, k0, k1,
+                 max_workgroups, (hipStream_t)stream_);
+}

@@ -1,0 +1,151 @@
+"""Root-mean-square norm over the last axis, with the residual's addition and its gradients, and its 8-bit output
+(csrc/rms_norm.hip).  Beside FrozenBatchNorm2d (statistics of maps) and the embeddings' L2 norm (sim_head/sim_net.py): the norm of
+activation rows, for heads of one's own between layers.linear.Linear layers.  No reference counterpart."""
+import math
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from .. import _lib as L
+
+_BF16 = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _rows(t, D):
+    """(rows, D) view with dense columns; a copy only where there is none."""
+    t = t.reshape(-1, D)
+    return t if D == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _check(what, x, weight, residual, eps):
+    L.need_gpu(x, weight, residual)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("%s: x has shape %s" % (what, tuple(x.shape)))
+    for name, t in (("x", x), ("weight", weight), ("residual", residual)):
+        if t is not None and t.dtype not in _BF16:
+            raise TypeError("%s: %s is %s (torch.float32 | torch.bfloat16)" % (what, name, t.dtype))
+        if t is not None and t.device != x.device:
+            raise ValueError("%s: %s is on %s, x on %s" % (what, name, t.device, x.device))
+    if weight is not None and tuple(weight.shape) != (x.shape[-1],):
+        raise ValueError("%s: weight has shape %s, x %s" % (what, tuple(weight.shape), tuple(x.shape)))
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError("%s: residual has shape %s, x %s" % (what, tuple(residual.shape), tuple(x.shape)))
+        if residual.dtype != x.dtype and residual.dtype != torch.float32:
+            raise TypeError("%s: residual is %s beside x in %s (x's type or torch.float32)" % (what, residual.dtype, x.dtype))
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError("%s: eps = %r" % (what, eps))
+
+
+def _types(x, residual, weight):
+    h = x if residual is None else residual
+    return _BF16[x.dtype] + 2 * _BF16[h.dtype] + (4 * _BF16[weight.dtype] if weight is not None else 0)
+
+
+def _forward(x, weight, residual, eps, want_rstd):
+    D = x.shape[-1]
+    x2 = _rows(x, D)
+    r2 = _rows(residual, D) if residual is not None else None
+    w = weight.contiguous() if weight is not None else None
+    R = x2.shape[0]
+    with torch.cuda.device(x.device):
+        y = torch.empty((R, D), dtype=x.dtype, device=x.device)
+        h = torch.empty((R, D), dtype=residual.dtype, device=x.device) if residual is not None else None
+        rstd = torch.empty(R, dtype=torch.float32, device=x.device) if want_rstd else None
+        L.check(L.lib().odw_rms_norm(L.ptr(x2), x2.stride(0), L.ptr(r2), r2.stride(0) if r2 is not None else 0, L.ptr(w), R, D, eps, L.ptr(y),
+                                     L.ptr(h), L.ptr(rstd), _types(x, residual, weight), L.stream()), "rms_norm")
+    return y.view(x.shape), h.view(x.shape) if h is not None else None, rstd
+
+
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, h, rstd = _forward(x, weight, residual, eps, True)
+        ctx.save_for_backward(x if h is None else h, weight, rstd)
+        ctx.dtypes = (x.dtype, None if residual is None else residual.dtype)
+        ctx.set_materialize_grads(False)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        x_type, h_type = ctx.dtypes
+        need_x, need_w, need_r = ctx.needs_input_grad[:3]
+        if dy is None:                                # only h was used
+            return (dh.to(x_type) if need_x and dh is not None else None, None if not need_w else torch.zeros_like(weight),
+                    dh if need_r else None, None)
+        D, shape = h.shape[-1], h.shape
+        h2, g2 = _rows(h, D), _rows(dy, D)
+        d2 = _rows(dh, D) if dh is not None else None
+        w = weight.contiguous() if weight is not None else None
+        R = h2.shape[0]
+        lib = L.lib()
+        with torch.cuda.device(h.device):
+            mixed = h_type is not None and h_type != x_type
+            dx = torch.empty((R, D), dtype=x_type, device=h.device) if need_x or (need_r and not mixed) else None
+            dres = torch.empty((R, D), dtype=h_type, device=h.device) if need_r and mixed else None
+            dw = torch.empty_like(w) if need_w else None
+            nbytes = lib.odw_rms_norm_bwd_workspace(R, D) if need_w else 0
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device) if need_w else None
+            types = _BF16[x_type] + 2 * _BF16[x_type if h_type is None else h_type] + (4 * _BF16[w.dtype] if w is not None else 0)
+            L.check(lib.odw_rms_norm_bwd(L.ptr(g2), g2.stride(0), L.ptr(d2), d2.stride(0) if d2 is not None else 0, L.ptr(h2), h2.stride(0),
+                                         L.ptr(w), L.ptr(rstd), R, D, L.ptr(dx), L.ptr(dres), L.ptr(dw), types, L.ptr(ws), nbytes,
+                                         L.stream()), "rms_norm_bwd")
+        dx = dx.view(shape) if dx is not None else None
+        if need_r:
+            dres = dres.view(shape) if mixed else dx
+        return dx if need_x else None, dw, dres if need_r else None, None
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-6):
+    """y = x / sqrt(mean(x^2) + eps) * weight over the last axis; with a residual (y, h): h = x + residual, y the norm of h.
+
+    x (..., D) fp32 or bf16, any row pitch; weight (D,) fp32 or bf16 or None; residual of x's shape, in x's type or fp32 (h has its
+    type; it is rounded once, and y is the norm of the rounded h).  Statistics and products are fp32, y is rounded once to x's type.
+    Gradients for x, weight and residual: the weight's summed over the rows in fp32, in one order.  h^2 has to fit fp32."""
+    _check("rms_norm", x, weight, residual, eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+        return _RMSNorm.apply(x, weight, residual, eps)
+    y, h, _ = _forward(x, weight, residual, eps, False)
+    return y if h is None else (y, h)
+
+
+@torch.no_grad()
+def rms_norm_fp8(x, weight=None, residual=None, eps=1e-6):
+    """rms_norm with its output in 8 bits: (q, scale), or (q, scale, h) with a residual.  q float8_e4m3fn of x's shape, scale fp32 (...,):
+    y ~ q.float() * scale[..., None], scale = max |y| / 448 of the row (2^-126 for a row of zeros); rounded to nearest even.  A row that
+    holds a NaN is all NaN.  No gradients."""
+    _check("rms_norm_fp8", x, weight, residual, eps)
+    D = x.shape[-1]
+    x2 = _rows(x, D)
+    r2 = _rows(residual, D) if residual is not None else None
+    w = weight.contiguous() if weight is not None else None
+    R = x2.shape[0]
+    with torch.cuda.device(x.device):
+        q = torch.empty((R, D), dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty(R, dtype=torch.float32, device=x.device)
+        h = torch.empty((R, D), dtype=residual.dtype, device=x.device) if residual is not None else None
+        L.check(L.lib().odw_rms_norm_fp8(L.ptr(x2), x2.stride(0), L.ptr(r2), r2.stride(0) if r2 is not None else 0, L.ptr(w), R, D, eps, L.ptr(q),
+                                         L.ptr(scale), L.ptr(h), _types(x, residual, weight), L.stream()), "rms_norm_fp8")
+    out = (q.view(x.shape), scale.view(x.shape[:-1]))
+    return out if h is None else out + (h.view(x.shape),)
+
+
+class RMSNorm(nn.Module):
+    """rms_norm with a gain of its own (ones): forward(x) -> y, forward(x, residual) -> (y, x + residual)."""
+
+    def __init__(self, dim, eps=1e-6, elementwise_affine=True):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim)) if elementwise_affine else None
+        self.dim = dim
+
+    def forward(self, x, residual=None):
+        if x.shape[-1] != self.dim:
+            raise ValueError("RMSNorm: x has %d columns, the norm %d" % (x.shape[-1], self.dim))
+        return rms_norm(x, self.weight, residual, self.eps)
+
+    def extra_repr(self):
+        return "%d, eps=%g" % (self.dim, self.eps)

@@ -1,0 +1,388 @@
+"""AdamW over many tensors at once, and the global gradient norm it is clipped by (csrc/adamw.hip).
+
+The reference trains with SGD only (solver/build.py:10-24, engine.FlatSGD here); this is the optimiser beside it, for heads
+that do not train well under SGD.  Three ways in:
+
+  * `SOLVER.OPTIMIZER "ADAMW"`: the training step of engine.build_training_step (tools/train_net.py) runs it over its flat buffers;
+  * `AdamW`, a torch.optim.Optimizer, for a module of one's own;
+  * `adamw_step` / `adamw8_step` / `grad_norm` / `clip_grad_norm_` on lists of tensors.
+
+States are fp32, or 8-bit floats (2 bytes a parameter for both averages instead of 8): the first average in float8_e4m3fn,
+the second in float8_e5m2, a power-of-two scale each for every 256 consecutive elements of a tensor, rounded stochastically with the
+counter-based stream of utils/rng.py -- a step is a function of its inputs and its key, whatever the launch geometry.
+
+Every tensor is on one GPU; the work goes to the current stream of that device; nothing is read back to the host."""
+import ctypes
+import math
+
+import torch
+
+from . import _lib as L
+from .utils import rng
+
+BLOCK = 256          # elements that share a scale of the 8-bit states
+# a gradient whose square is nothing in fp32 (below 1e-21) then moves p by at most lr * 1e-6, not by lr * g / eps of any size
+MIN_EPS = 1e-15
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _check_list(what, name, tensors, like, dtypes, n_of=lambda n: n):
+    """`tensors` beside `like`: as many, on the same GPU, contiguous, of one of `dtypes` and of matching size."""
+    if len(tensors) != len(like):
+        raise ValueError("%s: %d %s for %d tensors" % (what, len(tensors), name, len(like)))
+    device = like[0].device if like else None
+    for i, (t, p) in enumerate(zip(tensors, like)):
+        if t.device != device:
+            if not t.is_cuda:
+                L.need_gpu(t)
+            raise ValueError("%s: %s[%d] is on %s, tensor 0 on %s" % (what, name, i, t.device, device))
+        if t.dtype not in dtypes:
+            raise TypeError("%s: %s[%d] is %s (%s)" % (what, name, i, t.dtype, " | ".join(str(d) for d in dtypes)))
+        if not t.is_contiguous():
+            raise ValueError("%s: %s[%d] is not contiguous" % (what, name, i))
+        if t.numel() != n_of(p.numel()):
+            raise ValueError("%s: %s[%d] has %d elements, %d wanted" % (what, name, i, t.numel(), n_of(p.numel())))
+
+
+def _distinct(what, name, tensors):
+    """A tensor that is written must not be in the list twice (two workgroups would update it at once)."""
+    seen = [t.data_ptr() for t in tensors if t.numel()]
+    if len(set(seen)) != len(seen):
+        raise ValueError("%s: the same tensor is in `%s` twice" % (what, name))
+
+
+def _ptrs(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() if t is not None else 0 for t in tensors])
+
+
+def _sizes(tensors):
+    return (ctypes.c_int64 * len(tensors))(*[t.numel() for t in tensors])
+
+
+def _scalar_list(what, name, value, n):
+    if isinstance(value, (int, float)):
+        value = [value] * n
+    if len(value) != n:
+        raise ValueError("%s: %d values of %s for %d tensors" % (what, len(value), name, n))
+    for x in value:
+        if not (x >= 0.0 and math.isfinite(x)):
+            raise ValueError("%s: %s = %r" % (what, name, x))
+    return (ctypes.c_float * n)(*value)
+
+
+def _device_scalar(what, name, t, device, dtype):
+    if t.numel() != 1 or t.dtype != dtype or t.device != device:
+        raise ValueError("%s: %s has to be one %s on %s (got %s of %d elements on %s)" % (what, name, dtype, device, t.dtype, t.numel(), t.device))
+
+
+def _grads_of(what, items):
+    """Gradients out of a list of tensors and / or parameters: a leaf that requires grad stands for its .grad."""
+    grads = []
+    for t in items:
+        if t.requires_grad and t.is_leaf:
+            if t.grad is not None:
+                grads.append(t.grad)
+        else:
+            grads.append(t)
+    for i, g in enumerate(grads):
+        if g.is_sparse:
+            raise TypeError("%s: gradient %d is sparse" % (what, i))
+    return grads
+
+
+def _norm(what, grads, max_norm):
+    if not grads:
+        raise ValueError("%s: no gradients" % what)
+    L.need_gpu(grads[0])
+    _check_list(what, "grads", grads, grads, (torch.float32, torch.bfloat16))
+    if not max_norm > 0.0:
+        raise ValueError("%s: max_norm = %r" % (what, max_norm))
+    lib, n = L.lib(), _sizes(grads)
+    types = (ctypes.c_int * len(grads))(*[2 * _TYPES[g.dtype] for g in grads])
+    with torch.cuda.device(grads[0].device):
+        nbytes = lib.odw_grad_norm_workspace(len(grads), n)
+        ws = torch.empty(max(nbytes, 8), dtype=torch.uint8, device=grads[0].device)
+        out = torch.empty(2, dtype=torch.float32, device=grads[0].device)
+        L.check(lib.odw_grad_norm(len(grads), _ptrs(grads), n, types, float(max_norm), L.ptr(out), L.ptr(ws), nbytes, L.stream()), "grad_norm")
+    return out[0], out[1], n, types
+
+
+@torch.no_grad()
+def grad_norm(grads, max_norm=None):
+    """The 2-norm over all of `grads` (tensors, or parameters that stand for their .grad) as a 0-dim fp32 tensor; summed in fp64 in
+    one order, so the same from run to run.  With max_norm: (norm, coef), coef = min(1, max_norm / (norm + 1e-6)) -- the factor
+    that clips them, for `grad_scale` of adamw_step (clipping without a pass over the gradients).  Neither is read by the host.
+    A non-finite gradient makes the norm inf or NaN, and coef 0 or NaN."""
+    grads = [g if g.is_contiguous() else g.contiguous() for g in _grads_of("grad_norm", grads)]
+    norm, coef, _, _ = _norm("grad_norm", grads, math.inf if max_norm is None else max_norm)
+    return norm if max_norm is None else (norm, coef)
+
+
+@torch.no_grad()
+def clip_grad_norm_(grads, max_norm):
+    """Scale all of `grads` (tensors, or parameters that stand for their .grad) in place so that their common 2-norm is at most
+    max_norm; returns the norm before that (torch.nn.utils.clip_grad_norm_, without a host read)."""
+    grads = _grads_of("clip_grad_norm_", grads)
+    _distinct("clip_grad_norm_", "grads", grads)
+    norm, coef, n, types = _norm("clip_grad_norm_", grads, max_norm)
+    with torch.cuda.device(grads[0].device):
+        L.check(L.lib().odw_scale_tensors(len(grads), _ptrs(grads), n, types, L.ptr(coef), L.stream()), "scale_tensors")
+    torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_decay, grad_scale, copies, grad_mult, max_workgroups):
+    what = "adamw8_step" if bits8 else "adamw_step"
+    if not params:
+        return
+    L.need_gpu(params[0])
+    _check_list(what, "params", params, params, (torch.float32, torch.bfloat16))
+    _check_list(what, "grads", grads, params, (torch.float32, torch.bfloat16))
+    _check_list(what, "exp_avgs", m, params, (torch.float8_e4m3fn,) if bits8 else (torch.float32,))
+    _check_list(what, "exp_avg_sqs", v, params, (torch.float8_e5m2,) if bits8 else (torch.float32,))
+    written = [("params", params), ("exp_avgs", m), ("exp_avg_sqs", v)]
+    if bits8:
+        _check_list(what, "scales", scales, params, (torch.uint8,), lambda n: 2 * (-(-n // BLOCK)))
+        written.append(("scales", scales))
+    if copies is not None:
+        have = [c for c in copies if c is not None]
+        _check_list(what, "copies", [p if c is None else c for c, p in zip(copies, params)] if len(copies) == len(params) else copies,
+                    params, (torch.bfloat16, torch.float32))
+        if any(c.dtype != torch.bfloat16 for c in have):
+            raise TypeError("%s: copies are bfloat16" % what)
+        written.append(("copies", have))
+    for name, tensors in written:
+        _distinct(what, name, tensors)
+    count, device = len(params), params[0].device
+    if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+        raise ValueError("%s: betas = %r" % (what, betas))
+    if not (eps >= MIN_EPS and math.isfinite(eps)):
+        raise ValueError("%s: eps = %r" % (what, eps))
+    if not math.isfinite(grad_mult):
+        raise ValueError("%s: grad_mult = %r" % (what, grad_mult))
+    lr, weight_decay = _scalar_list(what, "lr", lr, count), _scalar_list(what, "weight_decay", weight_decay, count)
+    if grad_scale is not None:
+        _device_scalar(what, "grad_scale", grad_scale, device, torch.float32)
+    types = (ctypes.c_int * count)(*[_TYPES[p.dtype] + 2 * _TYPES[g.dtype] for p, g in zip(params, grads)])
+    lib, bias = L.lib(), None
+    with torch.cuda.device(device):
+        if torch.is_tensor(step):
+            _device_scalar(what, "step", step, device, torch.int64)
+            bias = torch.empty(4, dtype=torch.float32, device=device)
+            L.check(lib.odw_adamw_advance(L.ptr(step), betas[0], betas[1], L.ptr(bias), L.stream()), "adamw_advance")
+            torch.autograd.graph.increment_version([step])
+            number = 0
+        else:
+            number = int(step)
+            if number < 1 or number != step:
+                raise ValueError("%s: step = %r (the first one is 1)" % (what, step))
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("%s: a captured step would replay step %d for ever: pass `step` as an int64 tensor on the GPU" % (what, number))
+        tail = (_ptrs(copies) if copies is not None else None, _sizes(params), types, lr, weight_decay, betas[0], betas[1], eps, number,
+                L.ptr(bias), L.ptr(grad_scale), grad_mult)
+        head = (count, _ptrs(params), _ptrs(grads), _ptrs(m), _ptrs(v))
+        if bits8:
+            L.check(lib.odw_adamw8(*head, _ptrs(scales), *tail, key[0], key[1], max_workgroups, L.stream()), what)
+        else:
+            L.check(lib.odw_adamw(*head, *tail, max_workgroups, L.stream()), what)
+    for _, tensors in written:
+        torch.autograd.graph.increment_version(tensors)
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, grad_scale=None,
+               copies=None, grad_mult=1.0, max_workgroups=0):
+    """One AdamW step over lists of tensors, in place, one launch for up to 44 of them:
+
+        g' = g * grad_mult * grad_scale
+        m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
+        p -= lr (m / (1 - b1^step) / (sqrt(v / (1 - b2^step)) + eps) + weight_decay p)
+
+    params fp32 or bf16 (updated in fp32, rounded once to nearest), grads fp32 or bf16, states fp32; all contiguous, none twice in a
+    list, none overlapping.  lr, weight_decay: a number, or one per tensor.  step: the number of this step, from 1 -- or an int64
+    tensor on the GPU that holds the steps taken and is advanced here, the form a HIP graph can capture.  grad_scale: one fp32 on the
+    GPU (the clip coefficient of grad_norm).  copies: list of bf16 tensors (or None) that get the new params, as the matrix cores read
+    them.  max_workgroups: 0, or the width of a pass that runs beside other work."""
+    _step(False, params, grads, exp_avgs, exp_avg_sqs, None, step, None, lr, betas, eps, weight_decay, grad_scale, copies, grad_mult,
+          max_workgroups)
+
+
+@torch.no_grad()
+def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, scales, step, key, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                grad_scale=None, copies=None, grad_mult=1.0, max_workgroups=0):
+    """adamw_step with 8-bit states: exp_avgs float8_e4m3fn, exp_avg_sqs float8_e5m2, scales uint8 (ceil(n / 256), 2): exponent + 127 of
+    the power-of-two scales of the two averages of 256 elements; value = code * 2^(scale - 127) (state8_zeros, state8_read,
+    state8_write); a second average that is not zero is held as 2^-16 of its scale at least.  The update uses the averages before they are rounded.  key: two 32-bit integers, other ones every step
+    (utils.rng.stream_key(seed, step)); the random bits of an element depend on the key and on its position in the concatenation of
+    `params`.  With `step` on the GPU the step's number is added to key[1].  An average that is not finite is held as NaN."""
+    if len(key) != 2 or not all(0 <= int(k) < (1 << 32) for k in key):
+        raise ValueError("adamw8_step: key = %r (two 32-bit integers)" % (key,))
+    _step(True, params, grads, exp_avgs, exp_avg_sqs, scales, step, (int(key[0]), int(key[1])), lr, betas, eps, weight_decay, grad_scale,
+          copies, grad_mult, max_workgroups)
+
+
+# ---- the 8-bit states as tensors -----------------------------------------------------------------------------------------------------
+
+
+def state8_zeros(p):
+    """(exp_avg, exp_avg_sq, scales) of a parameter before its first step."""
+    blocks = -(-p.numel() // BLOCK)
+    return (torch.zeros(p.shape, dtype=torch.float8_e4m3fn, device=p.device), torch.zeros(p.shape, dtype=torch.float8_e5m2, device=p.device),
+            torch.full((blocks, 2), 1, dtype=torch.uint8, device=p.device))
+
+
+def state8_read(exp_avg, exp_avg_sq, scales):
+    """The two averages as fp32 tensors: exactly what is held."""
+    out = []
+    for col, q in enumerate((exp_avg, exp_avg_sq)):
+        s = (scales[:, col].to(torch.int32) << 23).view(torch.float32)          # (torch.ldexp goes through pow on the GPU: off by an ulp)
+        out.append((q.reshape(-1).float() * s.repeat_interleave(BLOCK)[:q.numel()]).view(q.shape))
+    return tuple(out)
+
+
+def state8_write(m, v, out=None):
+    """(exp_avg, exp_avg_sq, scales) that hold m and v, rounded to nearest; what state8_read gave comes back the same."""
+    res = state8_zeros(m) if out is None else out
+    for col, (x, q, top) in enumerate(((m, res[0], 8), (v, res[1], 15))):
+        n = x.numel()
+        blocks = torch.nn.functional.pad(x.detach().reshape(-1).float(), (0, -n % BLOCK)).view(-1, BLOCK)
+        finite = torch.isfinite(blocks)
+        a = torch.where(finite, blocks.abs(), torch.zeros_like(blocks)).amax(1)
+        bits = a.view(torch.int32)
+        e = ((bits >> 23) - top + ((bits & 0x7FFFFF) > 0x600000)).clamp(1, 254)
+        y = torch.where(finite, blocks * ((254 - e) << 23).view(torch.float32).view(-1, 1), torch.full_like(blocks, math.nan))
+        if col == 1:
+            y = torch.where(blocks > 0, y.clamp_min(2.0 ** -16), y)
+        q.copy_(y.view(-1)[:n].view(q.shape).to(q.dtype))
+        res[2][:, col] = e.to(torch.uint8)
+    return res
+
+
+# ---- the optimiser object ------------------------------------------------------------------------------------------------------------
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's arguments, groups and state names on the kernels above.
+
+    state_bits: 32, or 8.  max_grad_norm: clip the gradients' common 2-norm (over all groups) within the step.  seed: of the 8-bit
+    states' rounding.  capturable: the step's number lives on the GPU, so that step() can be captured into a HIP graph (learning
+    rates are then those of the capture).
+
+    state_dict() holds the averages in fp32 whatever state_bits is (an 8-bit state is read exactly and comes back the same), so
+    checkpoints move between 32 and 8 bits and torch.optim.AdamW."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None, seed=0,
+                 capturable=False):
+        if state_bits not in (8, 32):
+            raise ValueError("AdamW: state_bits = %r (8 | 32)" % (state_bits,))
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError("AdamW: max_grad_norm = %r" % (max_grad_norm,))
+        for name, x in (("lr", lr), ("weight_decay", weight_decay)):
+            if not (x >= 0.0 and math.isfinite(x)):
+                raise ValueError("AdamW: %s = %r" % (name, x))
+        if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError("AdamW: betas = %r" % (betas,))
+        if not (eps >= MIN_EPS and math.isfinite(eps)):
+            raise ValueError("AdamW: eps = %r" % (eps,))
+        self.state_bits, self.max_grad_norm, self.seed, self.capturable = state_bits, max_grad_norm, int(seed), bool(capturable)
+        self.grad_norm = None            # of the last step, where it was clipped (0-dim, on the GPU)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def _state(self, p):
+        st = self.state[p]
+        if not st:
+            if self.state_bits == 8:
+                st["exp_avg"], st["exp_avg_sq"], st["scales"] = state8_zeros(p)
+            else:
+                st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+                st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+            st["step"] = None            # (set by step(): a number, or with `capturable` a tensor that parameters share)
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        calls, grads, fresh = {}, [], {}
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise TypeError("AdamW: sparse gradient")
+                st = self._state(p)
+                if st["step"] is None:
+                    st["step"] = fresh.setdefault(p.device, torch.zeros(1, dtype=torch.int64, device=p.device)) if self.capturable else 0
+                g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
+                grads.append(g)
+                number = id(st["step"]) if self.capturable else st["step"]
+                calls.setdefault((tuple(group["betas"]), group["eps"], number), []).append((group, p, g, st))
+        if not grads:
+            return loss
+        coef = None
+        if self.max_grad_norm is not None:
+            self.grad_norm, coef = grad_norm(grads, self.max_grad_norm)
+        if self.capturable:
+            self._check_shared_steps(calls)
+        for ci, ((betas, eps, _), items) in enumerate(calls.items()):
+            step = items[0][3]["step"]
+            if not self.capturable:
+                step += 1
+            ps, gs = [x[1] for x in items], [x[2] for x in items]
+            m, v = ([x[3][k] for x in items] for k in ("exp_avg", "exp_avg_sq"))
+            more = dict(lr=[x[0]["lr"] for x in items], weight_decay=[x[0]["weight_decay"] for x in items], betas=betas, eps=eps, grad_scale=coef)
+            if self.state_bits == 8:
+                # (a step whose number is on the GPU adds it to the key there)
+                key = rng.stream_key(self.seed, (ci << 40) + (0 if self.capturable else step))
+                adamw8_step(ps, gs, m, v, [x[3]["scales"] for x in items], step, key, **more)
+            else:
+                adamw_step(ps, gs, m, v, step, **more)
+            if not self.capturable:
+                for x in items:
+                    x[3]["step"] = step
+        return loss
+
+    def _check_shared_steps(self, calls):
+        """Parameters that took their first step together share one counter on the GPU: it is advanced once, for all of them."""
+        have = [(x[3]["step"], x[1]) for items in calls.values() for x in items]
+        if len(set(id(s) for s, _ in have)) != len(calls):
+            raise RuntimeError("AdamW: capturable parameters that share a step counter have other betas or eps")
+        stepped = set(id(p) for _, p in have)
+        counters = set(id(s) for s, _ in have)
+        for p, st in self.state.items():
+            if id(st.get("step")) in counters and id(p) not in stepped:
+                raise RuntimeError("AdamW: a parameter without a gradient shares the step counter of others that have one (capturable)")
+
+    def state_dict(self):
+        """torch.optim.AdamW's layout: {"step": fp32 tensor, "exp_avg", "exp_avg_sq": fp32} a parameter."""
+        sd = super().state_dict()
+        for i, st in sd["state"].items():
+            m, v = st["exp_avg"], st["exp_avg_sq"]
+            if "scales" in st:
+                m, v = state8_read(m, v, st["scales"])
+            sd["state"][i] = {"step": torch.tensor(float(st["step"])), "exp_avg": m, "exp_avg_sq": v}
+        return sd
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """A state_dict() of this class (of either state_bits) or of torch.optim.AdamW."""
+        states = dict(state_dict["state"])
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        shared = {}
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        own = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, own):
+            if i not in states:
+                continue
+            step = int(states[i]["step"])
+            m, v = (states[i][k].detach().to(device=p.device, dtype=torch.float32).reshape(p.shape).contiguous() for k in ("exp_avg", "exp_avg_sq"))
+            st = self.state[p]
+            if self.state_bits == 8:
+                st["exp_avg"], st["exp_avg_sq"], st["scales"] = state8_write(m, v)
+            else:
+                st["exp_avg"], st["exp_avg_sq"] = m.clone(), v.clone()
+            st["step"] = step
+            if self.capturable:
+                st["step"] = shared.setdefault((p.device, step), torch.full((1,), step, dtype=torch.int64, device=p.device))
