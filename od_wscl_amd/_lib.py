@@ -6,6 +6,7 @@ written gfx950 kernels.  There is NO fallback: if the shared object is missing
 or a tensor is not on the GPU the call raises (the reference raises
 "Not implemented on the CPU" the same way, csrc/ROIPool.h:23).
 """
+import contextlib
 import ctypes
 import os
 
@@ -233,6 +234,16 @@ def stream():
     if _raw_stream is not None:
         return ctypes.c_void_p(_raw_stream(torch.cuda.current_device()))
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_no_guard = contextlib.nullcontext()
+
+
+def on_device_of(t):
+    """Context in which the current device is t's (launches go to the current device's current stream); nothing to do in the usual
+    case that it is already."""
+    index = t.get_device()
+    return _no_guard if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def ptr(t):

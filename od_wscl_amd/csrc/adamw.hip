@@ -13,9 +13,10 @@ namespace {
 constexpr int kMaxTensors = 44;          // (88 B each: the arguments stay under 4 KB)
 constexpr int kChunk = 4096;             // elements a workgroup handles at a time; a multiple of kBlock
 constexpr int kBlock = 256;              // elements that share a scale: one wave, four elements a lane
+constexpr int kNormChunk = 16384;        // the same of the norm: fewer partial sums for the workgroup that adds them
 constexpr int kThreads = 256;
 
-enum { kPBf16 = 1, kGBf16 = 2, kVec = 4 };
+enum { kPBf16 = 1, kGBf16 = 2 };
 
 struct Tensor {
     void* p;
@@ -66,69 +67,68 @@ __device__ __forceinline__ int find_tensor(F chunk0, int count, int c) {
     return lo;
 }
 
-// Four elements of a wave's 256: consecutive ones (vec: pointers aligned for it) or 64 apart.
-__device__ __forceinline__ int64_t elem(bool vec, int64_t base, int lane, int j) { return vec ? base + 4 * lane + j : base + lane + 64 * j; }
+// A wave's 256 elements, four consecutive ones a lane, by vectors declared with their element's alignment, which the memory instructions
+// take as well: tensors may start at any element.  Nothing is read twice: all loads and stores are marked nontemporal.
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned short us4 __attribute__((ext_vector_type(4)));
+typedef f4 f4_any __attribute__((aligned(4)));
+typedef us4 us4_any __attribute__((aligned(2)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
 
-__device__ __forceinline__ void load4(const void* src, bool bf16, bool vec, int64_t base, int lane, int64_t n, float (&x)[4]) {
-    if (vec && base + 4 * lane + 3 < n) {
-        if (bf16) {
-            const ushort4 u = *reinterpret_cast<const ushort4*>((const unsigned short*)src + base + 4 * lane);
-            x[0] = bf2f(u.x); x[1] = bf2f(u.y); x[2] = bf2f(u.z); x[3] = bf2f(u.w);
+// `left` = elements from src on (FULL: at least 256 -- nothing to check).
+template <bool BF, bool FULL>
+struct Four {
+    union { f4 f; us4 h; } u;
+    __device__ __forceinline__ void load(const void* src, int lane, int left) {
+        if (FULL) {
+            if (BF) u.h = __builtin_nontemporal_load((const us4_any*)src + lane);
+            else u.f = __builtin_nontemporal_load((const f4_any*)src + lane);
         } else {
-            const float4 u = *reinterpret_cast<const float4*>((const float*)src + base + 4 * lane);
-            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-        }
-        return;
-    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t i = elem(vec, base, lane, j);
-        x[j] = i < n ? (bf16 ? bf2f(((const unsigned short*)src)[i]) : ((const float*)src)[i]) : 0.0f;
+            for (int j = 0; j < 4; ++j) {
+                const int i = 4 * lane + j;
+                if (BF) u.h[j] = i < left ? ((const unsigned short*)src)[i] : (unsigned short)0;
+                else u.f[j] = i < left ? ((const float*)src)[i] : 0.0f;
+            }
+        }
     }
-}
-
-__device__ __forceinline__ void store4(void* dst, bool bf16, bool vec, int64_t base, int lane, int64_t n, const float (&x)[4]) {
-    if (vec && base + 4 * lane + 3 < n) {
-        if (bf16) {
-            ushort4 u;
-            u.x = f2bf(x[0]); u.y = f2bf(x[1]); u.z = f2bf(x[2]); u.w = f2bf(x[3]);
-            *reinterpret_cast<ushort4*>((unsigned short*)dst + base + 4 * lane) = u;
+    __device__ __forceinline__ float get(int j) const { return BF ? bf2f(u.h[j]) : u.f[j]; }
+    __device__ __forceinline__ void set(int j, float x) { if (BF) u.h[j] = f2bf(x); else u.f[j] = x; }
+    __device__ __forceinline__ void store(void* dst, int lane, int left) const {
+        if (FULL) {
+            if (BF) __builtin_nontemporal_store(u.h, (us4_any*)dst + lane);
+            else __builtin_nontemporal_store(u.f, (f4_any*)dst + lane);
         } else {
-            *reinterpret_cast<float4*>((float*)dst + base + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]);
-        }
-        return;
-    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t i = elem(vec, base, lane, j);
-        if (i < n) {
-            if (bf16) ((unsigned short*)dst)[i] = f2bf(x[j]);
-            else ((float*)dst)[i] = x[j];
+            for (int j = 0; j < 4; ++j) {
+                const int i = 4 * lane + j;
+                if (i >= left) continue;
+                if (BF) ((unsigned short*)dst)[i] = u.h[j];
+                else ((float*)dst)[i] = u.f[j];
+            }
         }
     }
-}
+};
 
-__device__ __forceinline__ uint32_t load4_u8(const uint8_t* src, bool vec, int64_t base, int lane, int64_t n) {
-    if (vec && base + 4 * lane + 3 < n) return *reinterpret_cast<const uint32_t*>(src + base + 4 * lane);
+template <bool FULL>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* src, int lane, int left) {
+    if (FULL) return __builtin_nontemporal_load((const u32_any*)src + lane);
     uint32_t u = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t i = elem(vec, base, lane, j);
-        if (i < n) u |= (uint32_t)src[i] << (8 * j);
-    }
+    for (int j = 0; j < 4; ++j)
+        if (4 * lane + j < left) u |= (uint32_t)src[4 * lane + j] << (8 * j);
     return u;
 }
 
-__device__ __forceinline__ void store4_u8(uint8_t* dst, bool vec, int64_t base, int lane, int64_t n, uint32_t u) {
-    if (vec && base + 4 * lane + 3 < n) {
-        *reinterpret_cast<uint32_t*>(dst + base + 4 * lane) = u;
+template <bool FULL>
+__device__ __forceinline__ void store_codes(uint8_t* dst, int lane, int left, uint32_t u) {
+    if (FULL) {
+        __builtin_nontemporal_store(u, (u32_any*)dst + lane);
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t i = elem(vec, base, lane, j);
-        if (i < n) dst[i] = (uint8_t)(u >> (8 * j));
-    }
+    for (int j = 0; j < 4; ++j)
+        if (4 * lane + j < left) dst[4 * lane + j] = (uint8_t)(u >> (8 * j));
 }
 
 // ---- the 8-bit states ---------------------------------------------------------------------------------------------------------
@@ -166,115 +166,144 @@ __device__ __forceinline__ int block_exponent(uint32_t mx) {
     return e < 1 ? 1 : e;
 }
 
-__device__ __forceinline__ float decode_m(uint32_t code, float scale) {
-    // sign | 7 bits: the normal numbers by rebiasing, the subnormal ones as the distance from 2^-6
-    const uint32_t a = code & 0x7Fu;
-    const bool low = a < 8u;
-    float x = __uint_as_float(((a + (low ? 8u : 0u)) << 20) + (120u << 23));
-    if (low) x -= 0.015625f;
-    if (a == 0x7Fu) x = __uint_as_float(0x7FC00000u);
-    x *= scale;
-    return (code & 0x80u) ? -x : x;
-}
-
-__device__ __forceinline__ float decode_v(uint32_t code, float scale) {
-    const uint32_t a = code & 0x7Fu;
-    const bool low = a < 4u;
-    float x = __uint_as_float(((a + (low ? 4u : 0u)) << 21) + (112u << 23));
-    if (low) x -= 6.103515625e-05f;
-    if (a >= 0x7Cu) x = __uint_as_float(a == 0x7Cu ? 0x7F800000u : 0x7FC00000u);
-    x *= scale;
-    return (code & 0x80u) ? -x : x;
-}
-
+// Largest of a wave's words, as a scalar: shifts within the rows of 16 lanes, then the rows' last lanes broadcast onwards.
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const uint32_t o = (uint32_t)__shfl_xor((int)x, off, 64);
-        x = x > o ? x : o;
+#define ODW_MAX_STEP(CTRL)                                                                              \
+    {                                                                                                   \
+        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);      \
+        x = x > o ? x : o;                                                                              \
     }
-    return x;
+    ODW_MAX_STEP(0x111) ODW_MAX_STEP(0x112) ODW_MAX_STEP(0x114) ODW_MAX_STEP(0x118)      // row_shr 1, 2, 4, 8
+    ODW_MAX_STEP(0x142) ODW_MAX_STEP(0x143)                                              // row_bcast 15, 31
+#undef ODW_MAX_STEP
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-// One pass: p, g, m, v in, p, m, v (and p's bf16 copy) out.  The averages are formed with one rounding an operation (no
-// contraction), in the order m b1 + g (1 - b1), v b2 + g g (1 - b2).
+struct Step { float gs, rc2, step, decay; uint32_t k1; };
+
+// p, g, m, v in, p, m, v (and p's bf16 copy) out, for U blocks of 256 elements `stride` apart: all loads first.  The averages are formed with
+// one rounding an operation (no contraction), in the order m b1 + g (1 - b1), v b2 + g g (1 - b2); the ratio with the hardware's root and
+// reciprocal (1 ulp each: 2^-22 of a step of lr is far below p's rounding; eps keeps the reciprocal's argument above 1e-15 and makes roots
+// of subnormal numbers, which the instruction takes for zero, irrelevant).
+template <bool BITS8, bool PBF, bool GBF, bool FULL, int U>
+__device__ __forceinline__ void update(const Args& a, const Tensor& t, const Step& s, int64_t base, int64_t stride, int lane, int left) {
+    Four<PBF, FULL> p[U];
+    Four<GBF, FULL> g[U];
+    Four<false, FULL> fm[U], fv[U];
+    uint32_t qm[U], qv[U], ee[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t o = base + u * stride;
+        p[u].load((const char*)t.p + o * (PBF ? 2 : 4), lane, left);
+        g[u].load((const char*)t.g + o * (GBF ? 2 : 4), lane, left);
+        if (BITS8) {
+            qm[u] = load_codes<FULL>((const uint8_t*)t.m + o, lane, left);
+            qv[u] = load_codes<FULL>((const uint8_t*)t.v + o, lane, left);
+            ee[u] = (uint32_t)t.e[2 * (o / kBlock)] | (uint32_t)t.e[2 * (o / kBlock) + 1] << 16;
+        } else {
+            fm[u].load((const float*)t.m + o, lane, left);
+            fv[u].load((const float*)t.v + o, lane, left);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t o = base + u * stride;
+        float m[4], v[4];
+        if (BITS8) {
+            const float sm = __uint_as_float((ee[u] & 0xFFu) << 23), sv = __uint_as_float((ee[u] >> 16) << 23);
+            const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)qm[u], false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)qm[u], true);
+            const auto v01 = __builtin_amdgcn_cvt_pk_f32_bf8((int)qv[u], false), v23 = __builtin_amdgcn_cvt_pk_f32_bf8((int)qv[u], true);
+            m[0] = m01[0] * sm; m[1] = m01[1] * sm; m[2] = m23[0] * sm; m[3] = m23[1] * sm;
+            v[0] = v01[0] * sv; v[1] = v01[1] * sv; v[2] = v23[0] * sv; v[3] = v23[1] * sv;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { m[j] = fm[u].get(j); v[j] = fv[u].get(j); }
+        }
+        Four<true, FULL> copy;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float gj = g[u].get(j) * s.gs, pj = p[u].get(j);
+            m[j] = m[j] * a.b1 + gj * a.omb1;
+            v[j] = v[j] * a.b2 + gj * gj * a.omb2;
+            const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[j]) * s.rc2 + a.eps);
+            p[u].set(j, pj - (s.step * m[j] * r + s.decay * pj));
+            copy.set(j, p[u].get(j));
+        }
+        p[u].store((char*)t.p + o * (PBF ? 2 : 4), lane, left);
+        if (t.copy) copy.store(t.copy + o, lane, left);
+        if (!BITS8) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { fm[u].set(j, m[j]); fv[u].set(j, v[j]); }
+            fm[u].store((float*)t.m + o, lane, left);
+            fv[u].store((float*)t.v + o, lane, left);
+            continue;
+        }
+        uint32_t mm = 0, mv = 0, bad = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            // (behind the end the loads gave zeros, and zeros they stay)
+            const uint32_t um = __float_as_uint(m[j]) & 0x7FFFFFFFu, uv = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+            if (um < 0x7F800000u) mm = mm > um ? mm : um; else bad = 1;
+            if (uv < 0x7F800000u) mv = mv > uv ? mv : uv; else bad = 1;
+        }
+        const int em = block_exponent<8>(wave_max(mm)), ev = block_exponent<15>(wave_max(mv));
+        const float im = __uint_as_float((uint32_t)(254 - em) << 23), iv = __uint_as_float((uint32_t)(254 - ev) << 23);
+        uint32_t om = 0, ov = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint64_t c = t.first + (uint64_t)o + (uint64_t)(4 * lane + j);
+            const uint32_t r = odw_mix(odw_mix((uint32_t)c ^ a.k0) + s.k1 + (uint32_t)(c >> 32));
+            om |= encode8<7, 3, 0>(m[j], im, r & 0xFFFFu, bad) << (8 * j);
+            ov |= encode8<15, 2, 1>(v[j], iv, r >> 16, bad) << (8 * j);
+        }
+        store_codes<FULL>((uint8_t*)t.m + o, lane, left, om);
+        store_codes<FULL>((uint8_t*)t.v + o, lane, left, ov);
+        if (lane == 0) {
+            t.e[2 * (o / kBlock)] = (uint8_t)em;
+            t.e[2 * (o / kBlock) + 1] = (uint8_t)ev;
+        }
+    }
+}
+
+constexpr int kUnroll = 2;
+
+// A chunk: its four waves take every fourth block, kUnroll at a time; the tensor's last, short block by itself.
+template <bool BITS8, bool PBF, bool GBF>
+__device__ __forceinline__ void chunk(const Args& a, const Tensor& t, const Step& s, int64_t begin, int wave, int lane) {
+    const int64_t rest = t.n - begin;
+    const int size = rest < kChunk ? (int)rest : kChunk, blocks = size / kBlock;
+    constexpr int kWaves = kThreads / 64;
+    int b = wave;
+    for (; b + (kUnroll - 1) * kWaves < blocks; b += kUnroll * kWaves)
+        update<BITS8, PBF, GBF, true, kUnroll>(a, t, s, begin + b * kBlock, kWaves * kBlock, lane, kBlock);
+    for (; b < blocks; b += kWaves) update<BITS8, PBF, GBF, true, 1>(a, t, s, begin + b * kBlock, 0, lane, kBlock);
+    if (b == blocks && size % kBlock) update<BITS8, PBF, GBF, false, 1>(a, t, s, begin + b * kBlock, 0, lane, size % kBlock);
+}
+
 template <bool BITS8>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const Args a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float c1 = a.c1, c2 = a.c2;
-    uint32_t k1 = a.k1;
+    Step s;
+    s.k1 = a.k1;
     if (a.bias) {
         c1 = a.bias[0];
         c2 = a.bias[1];
-        k1 += __float_as_uint(a.bias[2]);        // the step's number: a replayed launch draws new bits
+        s.k1 += __float_as_uint(a.bias[2]);        // the step's number: a replayed launch draws new bits
     }
-    const float gs = a.scale ? a.mult * *a.scale : a.mult;
-    const float rc2 = 1.0f / sqrtf(c2);
+    s.gs = a.scale ? a.mult * *a.scale : a.mult;
+    s.rc2 = 1.0f / sqrtf(c2);
     for (int c = blockIdx.x; c < a.chunks; c += gridDim.x) {
         const int ti = find_tensor([&](int i) { return a.t[i].chunk0; }, a.count, c);
         const Tensor& t = a.t[ti];
-        const int64_t n = t.n, c_begin = (int64_t)(c - t.chunk0) * kChunk;
-        const int64_t c_end = c_begin + kChunk < n ? c_begin + kChunk : n;
-        const bool vec = t.flags & kVec, pbf = t.flags & kPBf16, gbf = t.flags & kGBf16;
-        const float step = t.lr / c1, decay = t.lr * t.wd;
-        for (int64_t base = c_begin + wave * kBlock; base < c_end; base += (kThreads / 64) * kBlock) {
-            float p[4], g[4], m[4], v[4];
-            load4(t.p, pbf, vec, base, lane, n, p);
-            load4(t.g, gbf, vec, base, lane, n, g);
-            if (BITS8) {
-                const uint32_t um = load4_u8((const uint8_t*)t.m, vec, base, lane, n);
-                const uint32_t uv = load4_u8((const uint8_t*)t.v, vec, base, lane, n);
-                const uint8_t* e = t.e + 2 * (base / kBlock);
-                const float sm = __uint_as_float((uint32_t)e[0] << 23), sv = __uint_as_float((uint32_t)e[1] << 23);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    m[j] = decode_m(um >> (8 * j), sm);
-                    v[j] = decode_v(uv >> (8 * j), sv);
-                }
-            } else {
-                load4(t.m, false, vec, base, lane, n, m);
-                load4(t.v, false, vec, base, lane, n, v);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float gj = g[j] * gs;
-                m[j] = m[j] * a.b1 + gj * a.omb1;
-                v[j] = v[j] * a.b2 + gj * gj * a.omb2;
-                p[j] -= step * m[j] / (sqrtf(v[j]) * rc2 + a.eps) + decay * p[j];
-            }
-            store4(t.p, pbf, vec, base, lane, n, p);
-            if (t.copy) store4(t.copy, true, vec, base, lane, n, p);
-            if (!BITS8) {
-                store4(t.m, false, vec, base, lane, n, m);
-                store4(t.v, false, vec, base, lane, n, v);
-                continue;
-            }
-            uint32_t mm = 0, mv = 0, bad = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool in = elem(vec, base, lane, j) < n;
-                const uint32_t um = in ? __float_as_uint(m[j]) & 0x7FFFFFFFu : 0u, uv = in ? __float_as_uint(v[j]) & 0x7FFFFFFFu : 0u;
-                if (um < 0x7F800000u) mm = mm > um ? mm : um; else bad = 1;
-                if (uv < 0x7F800000u) mv = mv > uv ? mv : uv; else bad = 1;
-            }
-            mm = wave_max(mm);
-            mv = wave_max(mv);
-            const int em = block_exponent<8>(mm), ev = block_exponent<15>(mv);
-            const float im = __uint_as_float((uint32_t)(254 - em) << 23), iv = __uint_as_float((uint32_t)(254 - ev) << 23);
-            uint32_t qm = 0, qv = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint64_t at = t.first + (uint64_t)elem(vec, base, lane, j);
-                const uint32_t r = odw_mix(odw_mix((uint32_t)at ^ a.k0) + k1 + (uint32_t)(at >> 32));
-                qm |= encode8<7, 3, 0>(m[j], im, r & 0xFFFFu, bad) << (8 * j);
-                qv |= encode8<15, 2, 1>(v[j], iv, r >> 16, bad) << (8 * j);
-            }
-            store4_u8((uint8_t*)t.m, vec, base, lane, n, qm);
-            store4_u8((uint8_t*)t.v, vec, base, lane, n, qv);
-            if (lane == 0) {
-                t.e[2 * (base / kBlock)] = (uint8_t)em;
-                t.e[2 * (base / kBlock) + 1] = (uint8_t)ev;
-            }
+        const int64_t begin = (int64_t)(c - t.chunk0) * kChunk;
+        s.step = t.lr / c1;
+        s.decay = t.lr * t.wd;
+        switch (t.flags) {                         // (a tensor's types: uniform)
+            case 0: chunk<BITS8, false, false>(a, t, s, begin, wave, lane); break;
+            case kPBf16: chunk<BITS8, true, false>(a, t, s, begin, wave, lane); break;
+            case kGBf16: chunk<BITS8, false, true>(a, t, s, begin, wave, lane); break;
+            default: chunk<BITS8, true, true>(a, t, s, begin, wave, lane); break;
         }
     }
 }
@@ -290,21 +319,40 @@ __global__ void adamw_advance_kernel(int64_t* step, double b1, double b2, float*
 
 // ---- the global norm ------------------------------------------------------------------------------------------------------------
 // Sum of squares of a chunk: fp32 products exact in fp64, summed in fp64 in a fixed order.
+template <bool BF>
+__device__ __forceinline__ double sqsum(const void* g, int size, int wave, int lane) {
+    constexpr int kWaves = kThreads / 64, U = 8;
+    const int blocks = size / kBlock;
+    double s = 0.0;
+    int b = wave;
+    for (; b + (U - 1) * kWaves < blocks; b += U * kWaves) {
+        Four<BF, true> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u].load((const char*)g + (size_t)(b + u * kWaves) * kBlock * (BF ? 2 : 4), lane, kBlock);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s = fma((double)x[u].get(j), (double)x[u].get(j), s);
+    }
+    for (; b * kBlock < size; b += kWaves) {
+        Four<BF, false> x;
+        x.load((const char*)g + (size_t)b * kBlock * (BF ? 2 : 4), lane, size - b * kBlock);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s = fma((double)x.get(j), (double)x.get(j), s);
+    }
+    return s;
+}
+
 __global__ __launch_bounds__(kThreads) void sqsum_kernel(const NormArgs a, double* __restrict__ partial) {
     __shared__ double part[kThreads / 64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = blockIdx.x;
     const int ti = find_tensor([&](int i) { return a.chunk0[i]; }, a.count, c);
-    const int64_t n = a.n[ti], c_begin = (int64_t)(c - a.chunk0[ti]) * kChunk;
-    const int64_t c_end = c_begin + kChunk < n ? c_begin + kChunk : n;
-    const bool vec = a.flags[ti] & kVec, bf = a.flags[ti] & kGBf16;
-    double s = 0.0;
-    for (int64_t base = c_begin + wave * kBlock; base < c_end; base += (kThreads / 64) * kBlock) {
-        float g[4];
-        load4(a.g[ti], bf, vec, base, lane, n, g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s += (double)g[j] * (double)g[j];
-    }
+    const int64_t begin = (int64_t)(c - a.chunk0[ti]) * kNormChunk, rest = a.n[ti] - begin;
+    const int size = rest < kNormChunk ? (int)rest : kNormChunk;
+    const bool bf = a.flags[ti] & kGBf16;
+    const char* g = (const char*)a.g[ti] + begin * (bf ? 2 : 4);
+    double s = bf ? sqsum<true>(g, size, wave, lane) : sqsum<false>(g, size, wave, lane);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
     if (lane == 0) part[wave] = s;
@@ -317,6 +365,7 @@ __global__ __launch_bounds__(1024) void norm_finish_kernel(const double* __restr
                                                            float* __restrict__ out) {
     __shared__ double part[16];
     double s = 0.0;
+#pragma unroll 8
     for (int i = threadIdx.x; i < count; i += 1024) s += partial[i];
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
@@ -331,26 +380,47 @@ __global__ __launch_bounds__(1024) void norm_finish_kernel(const double* __restr
     }
 }
 
-__global__ __launch_bounds__(kThreads) void scale_kernel(const NormArgs a, const float* __restrict__ scale) {
-    const float s = *scale;
-    if (s == 1.0f) return;                       // the product would be what is there
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c = blockIdx.x;
-    const int ti = find_tensor([&](int i) { return a.chunk0[i]; }, a.count, c);
-    const int64_t n = a.n[ti], c_begin = (int64_t)(c - a.chunk0[ti]) * kChunk;
-    const int64_t c_end = c_begin + kChunk < n ? c_begin + kChunk : n;
-    const bool vec = a.flags[ti] & kVec, bf = a.flags[ti] & kGBf16;
-    for (int64_t base = c_begin + wave * kBlock; base < c_end; base += (kThreads / 64) * kBlock) {
-        float g[4];
-        load4(a.g[ti], bf, vec, base, lane, n, g);
+template <bool BF>
+__device__ __forceinline__ void scale(void* g, int size, int wave, int lane, float s) {
+    constexpr int kWaves = kThreads / 64, U = 4;
+    const int blocks = size / kBlock;
+    int b = wave;
+    for (; b + (U - 1) * kWaves < blocks; b += U * kWaves) {
+        Four<BF, true> x[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) g[j] *= s;
-        store4(const_cast<void*>(a.g[ti]), bf, vec, base, lane, n, g);
+        for (int u = 0; u < U; ++u) x[u].load((const char*)g + (size_t)(b + u * kWaves) * kBlock * (BF ? 2 : 4), lane, kBlock);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[u].set(j, x[u].get(j) * s);
+            x[u].store((char*)g + (size_t)(b + u * kWaves) * kBlock * (BF ? 2 : 4), lane, kBlock);
+        }
+    }
+    for (; b * kBlock < size; b += kWaves) {
+        Four<BF, false> x;
+        x.load((const char*)g + (size_t)b * kBlock * (BF ? 2 : 4), lane, size - b * kBlock);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.set(j, x.get(j) * s);
+        x.store((char*)g + (size_t)b * kBlock * (BF ? 2 : 4), lane, size - b * kBlock);
     }
 }
 
+__global__ __launch_bounds__(kThreads) void scale_kernel(const NormArgs a, const float* __restrict__ factor) {
+    const float s = *factor;
+    if (s == 1.0f) return;                       // the products would be what is there
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = blockIdx.x;
+    const int ti = find_tensor([&](int i) { return a.chunk0[i]; }, a.count, c);
+    const int64_t begin = (int64_t)(c - a.chunk0[ti]) * kNormChunk, rest = a.n[ti] - begin;
+    const int size = rest < kNormChunk ? (int)rest : kNormChunk;
+    const bool bf = a.flags[ti] & kGBf16;
+    char* g = (char*)const_cast<void*>(a.g[ti]) + begin * (bf ? 2 : 4);
+    if (bf) scale<true>(g, size, wave, lane, s);
+    else scale<false>(g, size, wave, lane, s);
+}
+
 bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
-int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+int64_t chunks_of(int64_t n, int chunk) { return (n + chunk - 1) / chunk; }
 constexpr int64_t kMaxElements = (int64_t)1 << 40;           // of one tensor: its chunks fit an int
 
 // Fills `a` with tensors from `i` on (empty ones left out) until it is full; returns the first one not taken.
@@ -358,13 +428,12 @@ int fill_norm_args(NormArgs& a, int i, int n_tensors, const void* const* g, cons
     a.count = a.chunks = 0;
     for (; i < n_tensors && a.count < kMaxTensors; ++i) {
         if (n[i] == 0) continue;
-        if (a.count && a.chunks + chunks_of(n[i]) > INT32_MAX) break;
-        const bool bf = types[i] & kGBf16;
+        if (a.count && a.chunks + chunks_of(n[i], kNormChunk) > INT32_MAX) break;
         a.g[a.count] = g[i];
         a.n[a.count] = n[i];
-        a.flags[a.count] = (uint8_t)((bf ? kGBf16 : 0) | (aligned(g[i], bf ? 8 : 16) ? kVec : 0));
+        a.flags[a.count] = (uint8_t)(types[i] & kGBf16);
         a.chunk0[a.count] = a.chunks;
-        a.chunks += (int)chunks_of(n[i]);
+        a.chunks += (int)chunks_of(n[i], kNormChunk);
         ++a.count;
     }
     return i;
@@ -412,17 +481,14 @@ int adamw(bool bits8, int n_tensors, void* const* p, const void* const* g, void*
         a.count = a.chunks = 0;
         for (; i < n_tensors && a.count < kMaxTensors; ++i) {
             if (n[i] == 0) continue;
-            if (a.count && a.chunks + chunks_of(n[i]) > INT32_MAX) break;
+            if (a.count && a.chunks + chunks_of(n[i], kChunk) > INT32_MAX) break;
             Tensor& t = a.t[a.count++];
             t.p = p[i]; t.g = g[i]; t.m = m[i]; t.v = v[i]; t.e = bits8 ? e[i] : nullptr;
             t.copy = copy ? (unsigned short*)copy[i] : nullptr;
             t.n = n[i]; t.first = first; t.lr = lr[i]; t.wd = wd[i];
-            const int sb = bits8 ? 4 : 16;
-            const bool vec = aligned(t.p, types[i] & kPBf16 ? 8 : 16) && aligned(t.g, types[i] & kGBf16 ? 8 : 16) && aligned(t.m, sb) &&
-                             aligned(t.v, sb) && aligned(t.copy, 8);
-            t.flags = types[i] | (vec ? kVec : 0);
+            t.flags = types[i];
             t.chunk0 = a.chunks;
-            a.chunks += (int)chunks_of(n[i]);
+            a.chunks += (int)chunks_of(n[i], kChunk);
             first += (uint64_t)n[i];
         }
         if (!a.count) break;
@@ -438,7 +504,7 @@ int adamw(bool bits8, int n_tensors, void* const* p, const void* const* g, void*
 
 ODW_EXPORT int64_t odw_grad_norm_workspace(int n_tensors, const int64_t* n) {
     int64_t chunks = 0;
-    for (int i = 0; i < n_tensors; ++i) chunks += n[i] > 0 ? chunks_of(n[i]) : 0;
+    for (int i = 0; i < n_tensors; ++i) chunks += n[i] > 0 ? chunks_of(n[i], kNormChunk) : 0;
     return chunks * (int64_t)sizeof(double);
 }
 

@@ -53,7 +53,297 @@ __device__ __forceinline__ uint32_t block_max(uint32_t x, uint32_t* part) {
 // e4m3, rounded to nearest even by the converter; |x| <= 448 or NaN (-> 0x7F).
 __device__ __forceinline__ uint8_t to_e4m3(float x) { return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false); }
 
-// A row a workgroup.
+// ---- rows that fit the registers ------------------------------------------------------------------------------------------------
+// TPR threads hold a row, VPT vectors of V elements each (16 bytes of x's type): one pass over memory, and between load and store the row's sum (and largest word) over the lanes -- by
+// cross-lane moves for TPR = 64, through LDS beyond.  Rows of any pitch, width and alignment go the
+// same way (the vector loads and stores are declared with their element's alignment, which the memory instructions take as well; a row's
+// last, short vector goes by elements): a row's result does not depend on where it lies.  The forms differ in TX (x, y, dy, dx) and TH (residual, h, dh, dresidual); the rest is
+// uniform branches.
+
+template <class T, int V> struct Vec {
+    typedef T full __attribute__((ext_vector_type(V)));
+    typedef full t __attribute__((aligned(sizeof(T))));
+};
+
+__device__ __forceinline__ float up(float x) { return x; }
+__device__ __forceinline__ float up(unsigned short x) { return __uint_as_float((uint32_t)x << 16); }
+template <class T> __device__ __forceinline__ T down(float x);
+template <> __device__ __forceinline__ float down<float>(float x) { return x; }
+template <> __device__ __forceinline__ unsigned short down<unsigned short>(float x) { return f2bf(x); }
+
+// `left` elements are there from src on.
+template <class T, int V>
+__device__ __forceinline__ void load(const T* src, int left, float (&x)[V]) {
+    if (left >= V) {
+        const typename Vec<T, V>::full u = *reinterpret_cast<const typename Vec<T, V>::t*>(src);
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = up((T)u[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = j < left ? up(src[j]) : 0.0f;
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ void store(T* dst, int left, const float (&x)[V]) {
+    if (left >= V) {
+        typename Vec<T, V>::full u;
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[j] = down<T>(x[j]);
+        *reinterpret_cast<typename Vec<T, V>::t*>(dst) = u;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < left) dst[j] = down<T>(x[j]);
+    }
+}
+template <int V>
+__device__ __forceinline__ void load_w(const void* w, bool bf, int i, int left, float (&x)[V]) {
+    if (!w) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = 1.0f;
+    } else if (bf) {
+        load<unsigned short, V>((const unsigned short*)w + i, left, x);
+    } else {
+        load<float, V>((const float*)w + i, left, x);
+    }
+}
+
+// Sum over the threads of a row.  `part` holds a number a wave and is written again by the next call: two barriers.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float x, float* part) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+    if constexpr (TPR > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = 0.0f;
+#pragma unroll
+        for (int k = 0; k < TPR / 64; ++k) x += part[k];
+    }
+    return x;
+}
+template <int TPR>
+__device__ __forceinline__ uint32_t row_max(uint32_t x, float* part) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const uint32_t o = (uint32_t)__shfl_xor((int)x, off, 64);
+        x = x > o ? x : o;
+    }
+    if constexpr (TPR > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = __uint_as_float(x);
+        __syncthreads();
+        x = 0;
+#pragma unroll
+        for (int k = 0; k < TPR / 64; ++k) {
+            const uint32_t o = __float_as_uint(part[k]);
+            x = x > o ? x : o;
+        }
+    }
+    return x;
+}
+
+template <class TX, class TH, int TPR, int VPT, int V>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_row_kernel(const TX* __restrict__ x, int64_t ldx, const TH* __restrict__ res,
+                                                                             int64_t ldr, const void* __restrict__ w, int64_t R, int D, float eps,
+                                                                             void* __restrict__ y, TH* __restrict__ h, float* __restrict__ rstd,
+                                                                             float* __restrict__ scale, int types) {
+    constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
+    __shared__ float part[TPR > 64 ? TPR / 64 : 1];
+    static_assert(TPR == 64 || kRows == 1, "rows that share a workgroup have a wave each");
+    const int t = kRows == 1 ? threadIdx.x : threadIdx.x % TPR;
+    // (a wave's row is uniform, and the compiler has to know it: scalar row addresses)
+    const int64_t r = kRows == 1 ? blockIdx.x : (int64_t)blockIdx.x * kRows + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+    if (r >= R) return;                          // (whole waves; with one row a workgroup never)
+    float v[VPT][V];
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int i = (k * TPR + t) * V;
+        if (i < D) {
+            load<TX, V>(x + r * ldx + i, D - i, v[k]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[k][j] = 0.0f;
+        }
+    }
+    if (res) {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int i = (k * TPR + t) * V;
+            if (i < D) {
+                float a[V];
+                load<TH, V>(res + r * ldr + i, D - i, a);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[k][j] = up(down<TH>(v[k][j] + a[j]));
+                store<TH, V>(h + r * D + i, D - i, v[k]);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) s += v[k][j] * v[k][j];
+    s = row_sum<TPR>(s, part);
+    const float rs = 1.0f / sqrtf(s / (float)D + eps);
+    if (rstd && t == 0) rstd[r] = rs;
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int i = (k * TPR + t) * V;
+        if (i < D) {
+            float g[V];
+            load_w<V>(w, types & kWBf16, i, D - i, g);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[k][j] = v[k][j] * rs * g[j];
+            if (!scale) {
+                store<TX, V>((TX*)y + r * D + i, D - i, v[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const uint32_t u = __float_as_uint(v[k][j]) & 0x7FFFFFFFu;
+                    top = top > u ? top : u;
+                }
+            }
+        }
+    }
+    if (!scale) return;
+    // the largest word of the magnitudes: a NaN's is above all numbers', so it makes the scale and the whole row NaN
+    const float sc0 = __uint_as_float(row_max<TPR>(top, part)) / 448.0f;
+    const float sc = sc0 < 1.17549435e-38f ? 1.17549435e-38f : sc0, inv = 1.0f / sc;
+    if (t == 0) scale[r] = sc;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int i = (k * TPR + t) * V;
+        if (i >= D) continue;
+        uint8_t* q = (uint8_t*)y + r * D + i;
+        typedef int word __attribute__((aligned(1)));
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][j] * inv, v[k][j + 1] * inv, 0, false);
+            u = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][j + 2] * inv, v[k][j + 3] * inv, u, true);
+            if (D - i >= j + 4) {
+                *reinterpret_cast<word*>(q + j) = u;
+            } else {
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    if (i + j + b < D) q[j + b] = (uint8_t)(u >> (8 * b));
+            }
+        }
+    }
+}
+
+// Rows blockIdx.x, + gridDim.x, ... of a workgroup (TPR = 64: of each of its four waves); the weight's gradient of those rows stays in
+// registers (of the widest rows, whose other numbers fill those, in LDS: each thread its own columns) and ends in a row of part_w of its
+// own, which rms_norm_dw_kernel sums in order.
+constexpr bool acc_in_lds(int tpr, int vpt, int v) { return tpr == 1024 && vpt * v >= 32; }
+template <class TX, class TH, int TPR, int VPT, int V>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_row_kernel(const TX* __restrict__ dy, int64_t ldy, const TH* __restrict__ dh,
+                                                                                 int64_t ldh, const TH* __restrict__ h, int64_t ldx,
+                                                                                 const void* __restrict__ w, const float* __restrict__ rstd, int64_t R,
+                                                                                 int D, TX* __restrict__ dx, TH* __restrict__ dres,
+                                                                                 float* __restrict__ part_w, int types) {
+    constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
+    __shared__ float part[TPR > 64 ? TPR / 64 : 1];
+    const int t = kRows == 1 ? threadIdx.x : threadIdx.x % TPR;
+    // (a wave's row is uniform, and the compiler has to know it: scalar row addresses)
+    const int own = kRows == 1 ? blockIdx.x : __builtin_amdgcn_readfirstlane(blockIdx.x * kRows + threadIdx.x / TPR);
+    constexpr bool kLds = acc_in_lds(TPR, VPT, V);
+    extern __shared__ float acc_lds[];           // kLds: VPT x TPR x V
+    float acc[kLds ? 1 : VPT][V];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (kLds) acc_lds[(k * TPR + t) * V + j] = 0.0f;
+            else acc[kLds ? 0 : k][j] = 0.0f;
+        }
+    for (int64_t r = own; r < R; r += (int64_t)gridDim.x * kRows) {
+        float g[VPT][V], v[VPT][V];
+        const float rs = rstd[r];
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int i = (k * TPR + t) * V;
+            if (i < D) {
+                load<TX, V>(dy + r * ldy + i, D - i, g[k]);
+                load<TH, V>(h + r * ldx + i, D - i, v[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) g[k][j] = v[k][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int i = (k * TPR + t) * V;
+            if (i < D) {
+                float wk[V];
+                load_w<V>(w, types & kWBf16, i, D - i, wk);
+                if (kLds) {
+                    auto* a = reinterpret_cast<typename Vec<float, V>::full*>(acc_lds) + k * TPR + t;
+                    typename Vec<float, V>::full sum = *a;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) sum[j] += g[k][j] * v[k][j] * rs;
+                    *a = sum;
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    if (!kLds) acc[kLds ? 0 : k][j] += g[k][j] * v[k][j] * rs;
+                    g[k][j] *= wk[j];
+                    s += g[k][j] * v[k][j];
+                }
+            }
+        }
+        s = row_sum<TPR>(s, part);
+        const float m = rs * rs * (s / (float)D);
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int i = (k * TPR + t) * V;
+            if (i >= D) continue;
+            float a[V];
+            if (dh) {
+                load<TH, V>(dh + r * ldh + i, D - i, a);
+#pragma unroll
+                for (int j = 0; j < V; ++j) a[j] += rs * (g[k][j] - v[k][j] * m);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) a[j] = rs * (g[k][j] - v[k][j] * m);
+            }
+            if (dx) store<TX, V>(dx + r * D + i, D - i, a);
+            if (dres) store<TH, V>(dres + r * D + i, D - i, a);
+        }
+    }
+    if (!part_w) return;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int i = (k * TPR + t) * V;
+        if (i < D) {
+            if (kLds) load<float, V>(acc_lds + (k * TPR + t) * V, V, acc[0]);
+            store<float, V>(part_w + (int64_t)own * D + i, D - i, acc[kLds ? 0 : k]);
+        }
+    }
+}
+
+// 64 columns a workgroup, the rows of part_w over its 16 waves.
+__global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restrict__ part_w, int G, int D, void* __restrict__ dw, int types) {
+    __shared__ float part[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.0f;
+    if (i < D)
+#pragma unroll 8
+        for (int g = wave; g < G; g += 16) s += part_w[(int64_t)g * D + i];
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && i < D) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) s += part[k][lane];
+        st(dw, types & kWBf16, i, s);
+    }
+}
+
+// ---- rows of any width: the workgroup walks a row as often as it needs it -------------------------------------------------------
 template <bool OUT8>
 __global__ __launch_bounds__(256) void rms_norm_kernel(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, int64_t R,
                                                        int D, float eps, void* y, void* h, float* rstd, float* scale, int types) {
@@ -116,21 +406,87 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(const void* dy, int64
     }
 }
 
-__global__ __launch_bounds__(256) void rms_norm_dw_kernel(const float* part_w, int G, int D, void* dw, int types) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= D) return;
-    float s = 0.0f;
-    for (int g = 0; g < G; ++g) s += part_w[(int64_t)g * D + i];
-    st(dw, types & kWBf16, i, s);
+// ---- which form ------------------------------------------------------------------------------------------------------------------
+template <int T_, int K_, int V_> struct Shape { static constexpr int tpr = T_, vpt = K_, v = V_; };
+template <class... S> struct Shapes {};
+
+// Rows by width, the first that holds one: a wave a row while a lane needs up to four vectors (no barrier), then 256 and 1024 threads.  The
+// backward pass keeps three numbers an element (gradient, h, the weight's gradient) instead of one: fewer elements a thread.
+typedef Shapes<Shape<64, 1, 4>, Shape<64, 2, 4>, Shape<64, 4, 4>, Shape<256, 2, 4>, Shape<256, 4, 4>, Shape<256, 8, 4>, Shape<1024, 4, 4>,
+               Shape<1024, 8, 4>> Fwd4;
+typedef Shapes<Shape<64, 1, 8>, Shape<64, 2, 8>, Shape<64, 4, 8>, Shape<256, 2, 8>, Shape<256, 4, 8>, Shape<256, 8, 8>, Shape<1024, 4, 8>> Fwd8;
+typedef Shapes<Shape<64, 1, 4>, Shape<64, 2, 4>, Shape<64, 4, 4>, Shape<256, 2, 4>, Shape<256, 4, 4>, Shape<1024, 2, 4>, Shape<1024, 4, 4>,
+               Shape<1024, 8, 4>> Bwd4;
+typedef Shapes<Shape<64, 1, 8>, Shape<64, 2, 8>, Shape<256, 1, 8>, Shape<256, 2, 8>, Shape<1024, 1, 8>, Shape<1024, 2, 8>, Shape<1024, 4, 8>> Bwd8;
+
+// f(shape) for the first shape that holds D elements; false where none does.
+template <class F, class... S>
+bool with_shape(int D, Shapes<S...>, F f) {
+    return ((D <= S::tpr * S::vpt * S::v ? (f(S()), true) : false) || ...);
 }
 
-constexpr int kBwdGroups = 512;
-int bwd_groups(int64_t R) { return (int)(R < kBwdGroups ? R : kBwdGroups); }
+// Row groups of the backward pass = rows of part_w: enough to fill the chip, few beside the rows.
+int bwd_groups(int64_t R, int D) {
+    const int most = D <= 1024 ? 1024 : D <= 4096 ? 512 : 256;
+    return (int)(R < most ? R : most);
+}
 
 int check(const char* what, int64_t R, int D, int types) {
     ODW_REQUIRE(R >= 0 && D >= 1, "%s: bad dims R=%lld D=%d", what, (long long)R, D);
     ODW_REQUIRE(types >= 0 && types < 8, "%s: bad types %d", what, types);
+    ODW_REQUIRE(!(types & kHBf16) || (types & kXBf16), "%s: bf16 rows h beside fp32 rows x", what);
     return ODW_OK;
+}
+
+template <class TX, class TH>
+void forward(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, int64_t R, int D, float eps, void* y, void* h, float* rstd,
+             float* scale, int types, hipStream_t stream) {
+    constexpr int V = sizeof(TX) == 2 ? 8 : 4;
+    auto launch = [&](auto s) {
+        typedef decltype(s) S;
+        constexpr int kRows = S::tpr > 256 ? 1 : 256 / S::tpr;
+        rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v><<<(unsigned)((R + kRows - 1) / kRows), kRows * S::tpr, 0, stream>>>(
+            (const TX*)x, ldx, (const TH*)res, ldr, w, R, D, eps, y, (TH*)h, rstd, scale, types);
+    };
+    if (R < ((int64_t)1 << 31)) {
+        if constexpr (V == 8) { if (with_shape(D, Fwd8(), launch)) return; }
+        else { if (with_shape(D, Fwd4(), launch)) return; }
+    }
+    const unsigned grid = (unsigned)(R < 65536 ? R : 65536);
+    if (scale) rms_norm_kernel<true><<<grid, 256, 0, stream>>>(x, ldx, res, ldr, w, R, D, eps, y, h, rstd, scale, types);
+    else rms_norm_kernel<false><<<grid, 256, 0, stream>>>(x, ldx, res, ldr, w, R, D, eps, y, h, rstd, scale, types);
+}
+
+// Returns the rows of part_w that were written.
+template <class TX, class TH>
+int backward(const void* dy, int64_t ldy, const void* dh, int64_t ldh, const void* h, int64_t ldx, const void* w, const float* rstd, int64_t R, int D,
+             void* dx, void* dres, float* part_w, int types, hipStream_t stream, hipError_t& status) {
+    constexpr int V = sizeof(TX) == 2 ? 8 : 4;
+    int groups = bwd_groups(R, D);
+    status = hipSuccess;
+    auto launch = [&](auto s) {
+        typedef decltype(s) S;
+        constexpr int kRows = S::tpr > 256 ? 1 : 256 / S::tpr;
+        const int grid = groups / kRows > 0 ? groups / kRows : 1;        // (R < kRows: the waves without a row leave zeros)
+        groups = grid * kRows;
+        const int lds = acc_in_lds(S::tpr, S::vpt, S::v) ? S::tpr * S::vpt * S::v * (int)sizeof(float) : 0;
+        const auto kernel = rms_norm_bwd_row_kernel<TX, TH, S::tpr, S::vpt, S::v>;
+        if (lds > 0) status = odw_set_max_lds(reinterpret_cast<const void*>(kernel), lds);
+        if (status != hipSuccess) return;
+        kernel<<<grid, kRows * S::tpr, lds, stream>>>(
+            (const TX*)dy, ldy, (const TH*)dh, ldh, (const TH*)h, ldx, w, rstd, R, D, (TX*)dx, (TH*)dres, part_w, types);
+    };
+    if constexpr (V == 8) { if (with_shape(D, Bwd8(), launch)) return groups; }
+    else { if (with_shape(D, Bwd4(), launch)) return groups; }
+    rms_norm_bwd_kernel<<<groups, 256, 0, stream>>>(dy, ldy, dh, ldh, h, ldx, w, rstd, R, D, dx, dres, part_w, types);
+    return groups;
+}
+
+template <class F>
+void by_types(int types, F f) {          // f(x's type, h's type)
+    if (!(types & kXBf16)) f(float(), float());
+    else if (types & kHBf16) f((unsigned short)0, (unsigned short)0);
+    else f((unsigned short)0, float());
 }
 
 }  // namespace
@@ -141,8 +497,9 @@ ODW_EXPORT int odw_rms_norm(const void* x, int64_t ld_x, const void* res, int64_
     if (rc != ODW_OK) return rc;
     if (R == 0) return ODW_OK;
     ODW_REQUIRE(x && y && (!res || h), "rms_norm: null pointer");
-    rms_norm_kernel<false><<<(unsigned)(R < 65536 ? R : 65536), 256, 0, (hipStream_t)stream_>>>(x, ld_x, res, ld_res, w, R, D, eps, y, h, rstd,
-                                                                                               nullptr, types);
+    by_types(types, [&](auto tx, auto th) {
+        forward<decltype(tx), decltype(th)>(x, ld_x, res, ld_res, w, R, D, eps, y, h, rstd, nullptr, types, (hipStream_t)stream_);
+    });
     ODW_CHECK_LAUNCH("rms_norm_kernel");
     return ODW_OK;
 }
@@ -153,13 +510,17 @@ ODW_EXPORT int odw_rms_norm_fp8(const void* x, int64_t ld_x, const void* res, in
     if (rc != ODW_OK) return rc;
     if (R == 0) return ODW_OK;
     ODW_REQUIRE(x && q && scale && (!res || h), "rms_norm_fp8: null pointer");
-    rms_norm_kernel<true><<<(unsigned)(R < 65536 ? R : 65536), 256, 0, (hipStream_t)stream_>>>(x, ld_x, res, ld_res, w, R, D, eps, q, h, nullptr,
-                                                                                              scale, types);
+    by_types(types, [&](auto tx, auto th) {
+        forward<decltype(tx), decltype(th)>(x, ld_x, res, ld_res, w, R, D, eps, q, h, nullptr, scale, types, (hipStream_t)stream_);
+    });
     ODW_CHECK_LAUNCH("rms_norm_kernel");
     return ODW_OK;
 }
 
-ODW_EXPORT int64_t odw_rms_norm_bwd_workspace(int64_t R, int D) { return (int64_t)bwd_groups(R) * D * (int64_t)sizeof(float); }
+// (+ 3: a workgroup of four rows writes four rows of part_w)
+ODW_EXPORT int64_t odw_rms_norm_bwd_workspace(int64_t R, int D) {
+    return R > 0 ? (int64_t)(bwd_groups(R, D) + 3) * D * (int64_t)sizeof(float) : 0;
+}
 
 ODW_EXPORT int odw_rms_norm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh, const void* h, int64_t ld_h, const void* w,
                                 const float* rstd, int64_t R, int D, void* dx, void* dres, void* dw, int types, void* workspace,
@@ -168,18 +529,23 @@ ODW_EXPORT int odw_rms_norm_bwd(const void* dy, int64_t ld_dy, const void* dh, i
     const int rc = check("rms_norm_bwd", R, D, types);
     if (rc != ODW_OK) return rc;
     ODW_REQUIRE(R == 0 || (dy && h && rstd), "rms_norm_bwd: null pointer");
-    if (dw && workspace_bytes < odw_rms_norm_bwd_workspace(R, D)) {
+    if (dw && R > 0 && workspace_bytes < odw_rms_norm_bwd_workspace(R, D)) {
         odw_set_error("rms_norm_bwd: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)odw_rms_norm_bwd_workspace(R, D));
         return ODW_EWORKSPACE;
     }
     ODW_REQUIRE(!dw || R == 0 || workspace, "rms_norm_bwd: null workspace");
-    const int G = bwd_groups(R);
+    int groups = 0;
+    hipError_t status = hipSuccess;
     if (R > 0) {
-        rms_norm_bwd_kernel<<<G, 256, 0, stream>>>(dy, ld_dy, dh, ld_dh, h, ld_h, w, rstd, R, D, dx, dres, dw ? (float*)workspace : nullptr, types);
+        by_types(types, [&](auto tx, auto th) {
+            groups = backward<decltype(tx), decltype(th)>(dy, ld_dy, dh, ld_dh, h, ld_h, w, rstd, R, D, dx, dres, dw ? (float*)workspace : nullptr,
+                                                          types, stream, status);
+        });
+        ODW_CHECK_HIP(status, "rms_norm_bwd attr");
         ODW_CHECK_LAUNCH("rms_norm_bwd_kernel");
     }
     if (dw) {
-        rms_norm_dw_kernel<<<(D + 255) / 256, 256, 0, stream>>>((const float*)workspace, G, D, dw, types);
+        rms_norm_dw_kernel<<<(unsigned)(((int64_t)D + 63) / 64), 1024, 0, stream>>>((const float*)workspace, groups, D, dw, types);
         ODW_CHECK_LAUNCH("rms_norm_dw_kernel");
     }
     return ODW_OK;

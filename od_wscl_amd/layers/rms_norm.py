@@ -14,20 +14,24 @@ _BF16 = {torch.float32: 0, torch.bfloat16: 1}
 
 def _rows(t, D):
     """(rows, D) view with dense columns; a copy only where there is none."""
-    t = t.reshape(-1, D)
-    return t if D == 1 or t.stride(1) == 1 else t.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, D)
+    return t if t.stride(1) == 1 or D == 1 else t.contiguous()
 
 
 def _check(what, x, weight, residual, eps):
     L.need_gpu(x, weight, residual)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("%s: x has shape %s" % (what, tuple(x.shape)))
+    device = x.get_device()
     for name, t in (("x", x), ("weight", weight), ("residual", residual)):
-        if t is not None and t.dtype not in _BF16:
+        if t is None:
+            continue
+        if t.dtype not in _BF16:
             raise TypeError("%s: %s is %s (torch.float32 | torch.bfloat16)" % (what, name, t.dtype))
-        if t is not None and t.device != x.device:
+        if t.get_device() != device:
             raise ValueError("%s: %s is on %s, x on %s" % (what, name, t.device, x.device))
-    if weight is not None and tuple(weight.shape) != (x.shape[-1],):
+    if weight is not None and (weight.dim() != 1 or weight.shape[0] != x.shape[-1]):
         raise ValueError("%s: weight has shape %s, x %s" % (what, tuple(weight.shape), tuple(x.shape)))
     if residual is not None:
         if residual.shape != x.shape:
@@ -49,7 +53,7 @@ def _forward(x, weight, residual, eps, want_rstd):
     r2 = _rows(residual, D) if residual is not None else None
     w = weight.contiguous() if weight is not None else None
     R = x2.shape[0]
-    with torch.cuda.device(x.device):
+    with L.on_device_of(x):
         y = torch.empty((R, D), dtype=x.dtype, device=x.device)
         h = torch.empty((R, D), dtype=residual.dtype, device=x.device) if residual is not None else None
         rstd = torch.empty(R, dtype=torch.float32, device=x.device) if want_rstd else None
@@ -82,7 +86,7 @@ class _RMSNorm(torch.autograd.Function):
         w = weight.contiguous() if weight is not None else None
         R = h2.shape[0]
         lib = L.lib()
-        with torch.cuda.device(h.device):
+        with L.on_device_of(h):
             mixed = h_type is not None and h_type != x_type
             dx = torch.empty((R, D), dtype=x_type, device=h.device) if need_x or (need_r and not mixed) else None
             dres = torch.empty((R, D), dtype=h_type, device=h.device) if need_r and mixed else None
@@ -123,7 +127,7 @@ def rms_norm_fp8(x, weight=None, residual=None, eps=1e-6):
     r2 = _rows(residual, D) if residual is not None else None
     w = weight.contiguous() if weight is not None else None
     R = x2.shape[0]
-    with torch.cuda.device(x.device):
+    with L.on_device_of(x):
         q = torch.empty((R, D), dtype=torch.float8_e4m3fn, device=x.device)
         scale = torch.empty(R, dtype=torch.float32, device=x.device)
         h = torch.empty((R, D), dtype=residual.dtype, device=x.device) if residual is not None else None

@@ -26,33 +26,42 @@ MIN_EPS = 1e-15
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
-def _check_list(what, name, tensors, like, dtypes, n_of=lambda n: n):
-    """`tensors` beside `like`: as many, on the same GPU, contiguous, of one of `dtypes` and of matching size."""
+def _check_list(what, name, tensors, like, dtypes, blocks=False):
+    """`tensors` beside `like`: as many, on the same GPU, contiguous, of one of `dtypes` and of matching size (`blocks`: two bytes for every
+    256 elements).  Returns their addresses."""
     if len(tensors) != len(like):
         raise ValueError("%s: %d %s for %d tensors" % (what, len(tensors), name, len(like)))
-    device = like[0].device if like else None
-    for i, (t, p) in enumerate(zip(tensors, like)):
-        if t.device != device:
-            if not t.is_cuda:
-                L.need_gpu(t)
-            raise ValueError("%s: %s[%d] is on %s, tensor 0 on %s" % (what, name, i, t.device, device))
-        if t.dtype not in dtypes:
-            raise TypeError("%s: %s[%d] is %s (%s)" % (what, name, i, t.dtype, " | ".join(str(d) for d in dtypes)))
-        if not t.is_contiguous():
+    device = like[0].get_device()
+    at = []
+    for t, p in zip(tensors, like):
+        n = p.numel()
+        if blocks:
+            n = 2 * (-(-n // BLOCK))
+        if t.get_device() != device or t.dtype not in dtypes or t.numel() != n or not t.is_contiguous():
+            i = len(at)
+            L.need_gpu(t)
+            if t.get_device() != device:
+                raise ValueError("%s: %s[%d] is on %s, tensor 0 on %s" % (what, name, i, t.device, like[0].device))
+            if t.dtype not in dtypes:
+                raise TypeError("%s: %s[%d] is %s (%s)" % (what, name, i, t.dtype, " | ".join(str(d) for d in dtypes)))
+            if t.numel() != n:
+                raise ValueError("%s: %s[%d] has %d elements, %d wanted" % (what, name, i, t.numel(), n))
             raise ValueError("%s: %s[%d] is not contiguous" % (what, name, i))
-        if t.numel() != n_of(p.numel()):
-            raise ValueError("%s: %s[%d] has %d elements, %d wanted" % (what, name, i, t.numel(), n_of(p.numel())))
+        at.append(t.data_ptr())
+    return at
 
 
-def _distinct(what, name, tensors):
-    """A tensor that is written must not be in the list twice (two workgroups would update it at once)."""
-    seen = [t.data_ptr() for t in tensors if t.numel()]
-    if len(set(seen)) != len(seen):
-        raise ValueError("%s: the same tensor is in `%s` twice" % (what, name))
+def _distinct(what, name, at):
+    """A tensor that is written must not be in the list twice (two workgroups would update it at once); empty ones have address 0."""
+    seen = set(at)
+    if len(seen) != len(at):
+        seen.discard(0)
+        if len(seen) != len(at) - at.count(0):
+            raise ValueError("%s: the same tensor is in `%s` twice" % (what, name))
 
 
-def _ptrs(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() if t is not None else 0 for t in tensors])
+def _ptrs(at):
+    return (ctypes.c_void_p * len(at))(*at)
 
 
 def _sizes(tensors):
@@ -90,21 +99,25 @@ def _grads_of(what, items):
     return grads
 
 
-def _norm(what, grads, max_norm):
+def _norm(what, grads, max_norm, written=False):
     if not grads:
         raise ValueError("%s: no gradients" % what)
     L.need_gpu(grads[0])
-    _check_list(what, "grads", grads, grads, (torch.float32, torch.bfloat16))
+    at = _check_list(what, "grads", grads, grads, (torch.float32, torch.bfloat16))
+    if written:
+        _distinct(what, "grads", at)
     if not max_norm > 0.0:
         raise ValueError("%s: max_norm = %r" % (what, max_norm))
-    lib, n = L.lib(), _sizes(grads)
+    lib, n, ptrs = L.lib(), _sizes(grads), _ptrs(at)
     types = (ctypes.c_int * len(grads))(*[2 * _TYPES[g.dtype] for g in grads])
-    with torch.cuda.device(grads[0].device):
+    with L.on_device_of(grads[0]):
         nbytes = lib.odw_grad_norm_workspace(len(grads), n)
-        ws = torch.empty(max(nbytes, 8), dtype=torch.uint8, device=grads[0].device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device) if nbytes else None
         out = torch.empty(2, dtype=torch.float32, device=grads[0].device)
-        L.check(lib.odw_grad_norm(len(grads), _ptrs(grads), n, types, float(max_norm), L.ptr(out), L.ptr(ws), nbytes, L.stream()), "grad_norm")
-    return out[0], out[1], n, types
+        L.check(lib.odw_grad_norm(len(grads), ptrs, n, types, float(max_norm), L.ptr(out), L.ptr(ws), nbytes, L.stream()), "grad_norm")
+        if written:
+            L.check(lib.odw_scale_tensors(len(grads), ptrs, n, types, ctypes.c_void_p(out.data_ptr() + 4), L.stream()), "scale_tensors")
+    return out
 
 
 @torch.no_grad()
@@ -114,8 +127,8 @@ def grad_norm(grads, max_norm=None):
     that clips them, for `grad_scale` of adamw_step (clipping without a pass over the gradients).  Neither is read by the host.
     A non-finite gradient makes the norm inf or NaN, and coef 0 or NaN."""
     grads = [g if g.is_contiguous() else g.contiguous() for g in _grads_of("grad_norm", grads)]
-    norm, coef, _, _ = _norm("grad_norm", grads, math.inf if max_norm is None else max_norm)
-    return norm if max_norm is None else (norm, coef)
+    out = _norm("grad_norm", grads, math.inf if max_norm is None else max_norm)
+    return out[0] if max_norm is None else (out[0], out[1])
 
 
 @torch.no_grad()
@@ -123,12 +136,9 @@ def clip_grad_norm_(grads, max_norm):
     """Scale all of `grads` (tensors, or parameters that stand for their .grad) in place so that their common 2-norm is at most
     max_norm; returns the norm before that (torch.nn.utils.clip_grad_norm_, without a host read)."""
     grads = _grads_of("clip_grad_norm_", grads)
-    _distinct("clip_grad_norm_", "grads", grads)
-    norm, coef, n, types = _norm("clip_grad_norm_", grads, max_norm)
-    with torch.cuda.device(grads[0].device):
-        L.check(L.lib().odw_scale_tensors(len(grads), _ptrs(grads), n, types, L.ptr(coef), L.stream()), "scale_tensors")
+    out = _norm("clip_grad_norm_", grads, max_norm, written=True)
     torch.autograd.graph.increment_version(grads)
-    return norm
+    return out[0]
 
 
 def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_decay, grad_scale, copies, grad_mult, max_workgroups):
@@ -136,23 +146,25 @@ def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_
     if not params:
         return
     L.need_gpu(params[0])
-    _check_list(what, "params", params, params, (torch.float32, torch.bfloat16))
-    _check_list(what, "grads", grads, params, (torch.float32, torch.bfloat16))
-    _check_list(what, "exp_avgs", m, params, (torch.float8_e4m3fn,) if bits8 else (torch.float32,))
-    _check_list(what, "exp_avg_sqs", v, params, (torch.float8_e5m2,) if bits8 else (torch.float32,))
-    written = [("params", params), ("exp_avgs", m), ("exp_avg_sqs", v)]
+    floats = (torch.float32, torch.bfloat16)
+    ap, ag = _check_list(what, "params", params, params, floats), _check_list(what, "grads", grads, params, floats)
+    am = _check_list(what, "exp_avgs", m, params, (torch.float8_e4m3fn,) if bits8 else (torch.float32,))
+    av = _check_list(what, "exp_avg_sqs", v, params, (torch.float8_e5m2,) if bits8 else (torch.float32,))
+    written = [("params", params, ap), ("exp_avgs", m, am), ("exp_avg_sqs", v, av)]
     if bits8:
-        _check_list(what, "scales", scales, params, (torch.uint8,), lambda n: 2 * (-(-n // BLOCK)))
-        written.append(("scales", scales))
+        ae = _check_list(what, "scales", scales, params, (torch.uint8,), blocks=True)
+        written.append(("scales", scales, ae))
+    ac = None
     if copies is not None:
-        have = [c for c in copies if c is not None]
-        _check_list(what, "copies", [p if c is None else c for c, p in zip(copies, params)] if len(copies) == len(params) else copies,
-                    params, (torch.bfloat16, torch.float32))
-        if any(c.dtype != torch.bfloat16 for c in have):
-            raise TypeError("%s: copies are bfloat16" % what)
-        written.append(("copies", have))
-    for name, tensors in written:
-        _distinct(what, name, tensors)
+        if len(copies) != len(params):
+            raise ValueError("%s: %d copies for %d tensors" % (what, len(copies), len(params)))
+        have = [(c, p) for c, p in zip(copies, params) if c is not None]
+        at = _check_list(what, "copies", [c for c, _ in have], [p for _, p in have], (torch.bfloat16,)) if have else []
+        written.append(("copies", [c for c, _ in have], at))
+        at = iter(at)
+        ac = [0 if c is None else next(at) for c in copies]
+    for name, _, at in written:
+        _distinct(what, name, at)
     count, device = len(params), params[0].device
     if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
         raise ValueError("%s: betas = %r" % (what, betas))
@@ -165,7 +177,7 @@ def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_
         _device_scalar(what, "grad_scale", grad_scale, device, torch.float32)
     types = (ctypes.c_int * count)(*[_TYPES[p.dtype] + 2 * _TYPES[g.dtype] for p, g in zip(params, grads)])
     lib, bias = L.lib(), None
-    with torch.cuda.device(device):
+    with L.on_device_of(params[0]):
         if torch.is_tensor(step):
             _device_scalar(what, "step", step, device, torch.int64)
             bias = torch.empty(4, dtype=torch.float32, device=device)
@@ -178,14 +190,14 @@ def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_
                 raise ValueError("%s: step = %r (the first one is 1)" % (what, step))
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("%s: a captured step would replay step %d for ever: pass `step` as an int64 tensor on the GPU" % (what, number))
-        tail = (_ptrs(copies) if copies is not None else None, _sizes(params), types, lr, weight_decay, betas[0], betas[1], eps, number,
+        tail = (_ptrs(ac) if ac is not None else None, _sizes(params), types, lr, weight_decay, betas[0], betas[1], eps, number,
                 L.ptr(bias), L.ptr(grad_scale), grad_mult)
-        head = (count, _ptrs(params), _ptrs(grads), _ptrs(m), _ptrs(v))
+        head = (count, _ptrs(ap), _ptrs(ag), _ptrs(am), _ptrs(av))
         if bits8:
-            L.check(lib.odw_adamw8(*head, _ptrs(scales), *tail, key[0], key[1], max_workgroups, L.stream()), what)
+            L.check(lib.odw_adamw8(*head, _ptrs(ae), *tail, key[0], key[1], max_workgroups, L.stream()), what)
         else:
             L.check(lib.odw_adamw(*head, *tail, max_workgroups, L.stream()), what)
-    for _, tensors in written:
+    for _, tensors, _ in written:
         torch.autograd.graph.increment_version(tensors)
 
 
