@@ -71,17 +71,20 @@ template <class T> __device__ __forceinline__ T down(float x);
 template <> __device__ __forceinline__ float down<float>(float x) { return x; }
 template <> __device__ __forceinline__ unsigned short down<unsigned short>(float x) { return f2bf(x); }
 
-// `left` elements are there from src on.
+// `left` elements are there from src on.  fetch() leaves the words as they are (nothing waits for them until they are used).
+template <class T, int V>
+__device__ __forceinline__ typename Vec<T, V>::full fetch(const T* src, int left) {
+    if (left >= V) return *reinterpret_cast<const typename Vec<T, V>::t*>(src);
+    typename Vec<T, V>::full u;
+#pragma unroll
+    for (int j = 0; j < V; ++j) u[j] = j < left ? src[j] : (T)0;
+    return u;
+}
 template <class T, int V>
 __device__ __forceinline__ void load(const T* src, int left, float (&x)[V]) {
-    if (left >= V) {
-        const typename Vec<T, V>::full u = *reinterpret_cast<const typename Vec<T, V>::t*>(src);
+    const typename Vec<T, V>::full u = fetch<T, V>(src, left);
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = up((T)u[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = j < left ? up(src[j]) : 0.0f;
-    }
+    for (int j = 0; j < V; ++j) x[j] = up((T)u[j]);
 }
 template <class T, int V>
 __device__ __forceinline__ void store(T* dst, int left, const float (&x)[V]) {
@@ -108,13 +111,13 @@ __device__ __forceinline__ void load_w(const void* w, bool bf, int i, int left, 
     }
 }
 
-// Sum over the threads of a row.  `part` holds a number a wave and is written again by the next call: two barriers.
+// Sum over the threads of a row.  `part` holds a number a wave; the next call but one may use it again (a thread that writes it then has
+// passed the barrier of the call between, which every reader of this one has reached).
 template <int TPR>
 __device__ __forceinline__ float row_sum(float x, float* part) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
     if constexpr (TPR > 64) {
-        __syncthreads();
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
         __syncthreads();
         x = 0.0f;
@@ -131,7 +134,6 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x, float* part) {
         x = x > o ? x : o;
     }
     if constexpr (TPR > 64) {
-        __syncthreads();
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = __uint_as_float(x);
         __syncthreads();
         x = 0;
@@ -150,7 +152,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_row_kernel(con
                                                                              void* __restrict__ y, TH* __restrict__ h, float* __restrict__ rstd,
                                                                              float* __restrict__ scale, int types) {
     constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
-    __shared__ float part[TPR > 64 ? TPR / 64 : 1];
+    __shared__ float part[2][TPR > 64 ? TPR / 64 : 1];
     static_assert(TPR == 64 || kRows == 1, "rows that share a workgroup have a wave each");
     const int t = kRows == 1 ? threadIdx.x : threadIdx.x % TPR;
     // (a wave's row is uniform, and the compiler has to know it: scalar row addresses)
@@ -185,7 +187,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_row_kernel(con
     for (int k = 0; k < VPT; ++k)
 #pragma unroll
         for (int j = 0; j < V; ++j) s += v[k][j] * v[k][j];
-    s = row_sum<TPR>(s, part);
+    s = row_sum<TPR>(s, part[0]);
     const float rs = 1.0f / sqrtf(s / (float)D + eps);
     if (rstd && t == 0) rstd[r] = rs;
     uint32_t top = 0;
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_row_kernel(con
     }
     if (!scale) return;
     // the largest word of the magnitudes: a NaN's is above all numbers', so it makes the scale and the whole row NaN
-    const float sc0 = __uint_as_float(row_max<TPR>(top, part)) / 448.0f;
+    const float sc0 = __uint_as_float(row_max<TPR>(top, part[1])) / 448.0f;
     const float sc = sc0 < 1.17549435e-38f ? 1.17549435e-38f : sc0, inv = 1.0f / sc;
     if (t == 0) scale[r] = sc;
 #pragma unroll
@@ -235,9 +237,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_row_kernel(con
 }
 
 // Rows blockIdx.x, + gridDim.x, ... of a workgroup (TPR = 64: of each of its four waves); the weight's gradient of those rows stays in
-// registers (of the widest rows, whose other numbers fill those, in LDS: each thread its own columns) and ends in a row of part_w of its
-// own, which rms_norm_dw_kernel sums in order.
-constexpr bool acc_in_lds(int tpr, int vpt, int v) { return tpr == 1024 && vpt * v >= 32; }
+// registers and ends in a row of part_w of its own, which rms_norm_dw_kernel sums in order.  While a row's sum goes round, the loads of the next
+// row are in flight (kAhead): few groups of rows (little part_w) keep the memory busy.  1024 threads have half the registers each: rows over
+// 8 elements a thread are loaded when they are due there, and of the widest ones the weight's gradient lies in LDS (each thread its own
+// columns).
+constexpr bool wide_row(int tpr, int vpt, int v) { return tpr == 1024 && vpt * v >= 32; }
+
 template <class TX, class TH, int TPR, int VPT, int V>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_row_kernel(const TX* __restrict__ dy, int64_t ldy, const TH* __restrict__ dh,
                                                                                  int64_t ldh, const TH* __restrict__ h, int64_t ldx,
@@ -245,71 +250,92 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_row_kernel
                                                                                  int D, TX* __restrict__ dx, TH* __restrict__ dres,
                                                                                  float* __restrict__ part_w, int types) {
     constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
-    __shared__ float part[TPR > 64 ? TPR / 64 : 1];
+    constexpr bool kWide = wide_row(TPR, VPT, V), kAhead = TPR <= 256 || VPT * V <= 8;
+    __shared__ float part[2][TPR > 64 ? TPR / 64 : 1];
+    extern __shared__ float acc_lds[];           // kWide: VPT x TPR x V
+    typedef typename Vec<float, V>::full Sum;
     const int t = kRows == 1 ? threadIdx.x : threadIdx.x % TPR;
     // (a wave's row is uniform, and the compiler has to know it: scalar row addresses)
     const int own = kRows == 1 ? blockIdx.x : __builtin_amdgcn_readfirstlane(blockIdx.x * kRows + threadIdx.x / TPR);
-    constexpr bool kLds = acc_in_lds(TPR, VPT, V);
-    extern __shared__ float acc_lds[];           // kLds: VPT x TPR x V
-    float acc[kLds ? 1 : VPT][V];
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    Sum acc[kWide ? 1 : VPT], wk[kWide ? 1 : VPT];
+    Sum* wide_acc = reinterpret_cast<Sum*>(acc_lds);
+    typename Vec<TX, V>::full g[VPT], g_next[kAhead ? VPT : 1];
+    typename Vec<TH, V>::full v[VPT], v_next[kAhead ? VPT : 1];
+    const void* w_now = w;                       // (see the loop)
+    auto weight = [&](int k, float (&x)[V]) {
+        const int i = (k * TPR + t) * V;
+        if (kWide) {
+            load_w<V>(w_now, types & kWBf16, i, D - i, x);
+        } else {
 #pragma unroll
-    for (int k = 0; k < VPT; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            if (kLds) acc_lds[(k * TPR + t) * V + j] = 0.0f;
-            else acc[kLds ? 0 : k][j] = 0.0f;
+            for (int j = 0; j < V; ++j) x[j] = wk[kWide ? 0 : k][j];
         }
-    for (int64_t r = own; r < R; r += (int64_t)gridDim.x * kRows) {
-        float g[VPT][V], v[VPT][V];
+    };
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int i = (k * TPR + t) * V;
+        if (kWide) {
+            wide_acc[k * TPR + t] = (Sum)0.0f;
+        } else {
+            float x[V];
+            load_w<V>(w, types & kWBf16, i, D - i, x);
+            acc[kWide ? 0 : k] = (Sum)0.0f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) wk[kWide ? 0 : k][j] = x[j];
+        }
+        if (kAhead && own < R) {
+            g_next[kAhead ? k : 0] = fetch<TX, V>(dy + own * ldy + i, D - i);
+            v_next[kAhead ? k : 0] = fetch<TH, V>(h + own * ldx + i, D - i);
+        }
+    }
+    int turn = 0;
+    for (int64_t r = own; r < R; r += step, turn ^= 1) {
         const float rs = rstd[r];
+        const int64_t next = r + step < R ? r + step : r;
+        if (kWide) asm volatile("" : "+s"(w_now));       // loads of w stay in the loop: kept across rows they would not fit the registers
+        typename Vec<TH, V>::full d[kAhead ? VPT : 1];
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int i = (k * TPR + t) * V;
+            if (kAhead) {
+                g[k] = g_next[kAhead ? k : 0];
+                v[k] = v_next[kAhead ? k : 0];
+                if (dh) d[kAhead ? k : 0] = fetch<TH, V>(dh + r * ldh + i, D - i);
+                g_next[kAhead ? k : 0] = fetch<TX, V>(dy + next * ldy + i, D - i);
+                v_next[kAhead ? k : 0] = fetch<TH, V>(h + next * ldx + i, D - i);
+            } else {
+                g[k] = fetch<TX, V>(dy + r * ldy + i, D - i);
+                v[k] = fetch<TH, V>(h + r * ldx + i, D - i);
+            }
+        }
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int i = (k * TPR + t) * V;
-            if (i < D) {
-                load<TX, V>(dy + r * ldy + i, D - i, g[k]);
-                load<TH, V>(h + r * ldx + i, D - i, v[k]);
-            } else {
+            Sum a = kWide ? wide_acc[k * TPR + t] : acc[kWide ? 0 : k];
+            float x[V];
+            weight(k, x);
 #pragma unroll
-                for (int j = 0; j < V; ++j) g[k][j] = v[k][j] = 0.0f;
+            for (int j = 0; j < V; ++j) {
+                const float gj = up((TX)g[k][j]), vj = up((TH)v[k][j]);
+                a[j] += gj * vj * rs;
+                s += gj * x[j] * vj;
             }
+            if (kWide) wide_acc[k * TPR + t] = a;
+            else acc[kWide ? 0 : k] = a;
         }
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            const int i = (k * TPR + t) * V;
-            if (i < D) {
-                float wk[V];
-                load_w<V>(w, types & kWBf16, i, D - i, wk);
-                if (kLds) {
-                    auto* a = reinterpret_cast<typename Vec<float, V>::full*>(acc_lds) + k * TPR + t;
-                    typename Vec<float, V>::full sum = *a;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) sum[j] += g[k][j] * v[k][j] * rs;
-                    *a = sum;
-                }
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    if (!kLds) acc[kLds ? 0 : k][j] += g[k][j] * v[k][j] * rs;
-                    g[k][j] *= wk[j];
-                    s += g[k][j] * v[k][j];
-                }
-            }
-        }
-        s = row_sum<TPR>(s, part);
+        s = row_sum<TPR>(s, part[turn]);
         const float m = rs * rs * (s / (float)D);
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             const int i = (k * TPR + t) * V;
             if (i >= D) continue;
-            float a[V];
-            if (dh) {
-                load<TH, V>(dh + r * ldh + i, D - i, a);
+            if (!kAhead && dh) d[0] = fetch<TH, V>(dh + r * ldh + i, D - i);
+            float x[V], a[V];
+            weight(k, x);
 #pragma unroll
-                for (int j = 0; j < V; ++j) a[j] += rs * (g[k][j] - v[k][j] * m);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) a[j] = rs * (g[k][j] - v[k][j] * m);
-            }
+            for (int j = 0; j < V; ++j)
+                a[j] = rs * (up((TX)g[k][j]) * x[j] - up((TH)v[k][j]) * m) + (dh ? up((TH)d[kAhead ? k : 0][j]) : 0.0f);
             if (dx) store<TX, V>(dx + r * D + i, D - i, a);
             if (dres) store<TH, V>(dres + r * D + i, D - i, a);
         }
@@ -318,10 +344,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_row_kernel
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         const int i = (k * TPR + t) * V;
-        if (i < D) {
-            if (kLds) load<float, V>(acc_lds + (k * TPR + t) * V, V, acc[0]);
-            store<float, V>(part_w + (int64_t)own * D + i, D - i, acc[kLds ? 0 : k]);
-        }
+        if (i >= D) continue;
+        const Sum a = kWide ? wide_acc[k * TPR + t] : acc[kWide ? 0 : k];
+        float x[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = a[j];
+        store<float, V>(part_w + (int64_t)own * D + i, D - i, x);
     }
 }
 
@@ -469,7 +497,7 @@ int backward(const void* dy, int64_t ldy, const void* dh, int64_t ldh, const voi
         constexpr int kRows = S::tpr > 256 ? 1 : 256 / S::tpr;
         const int grid = groups / kRows > 0 ? groups / kRows : 1;        // (R < kRows: the waves without a row leave zeros)
         groups = grid * kRows;
-        const int lds = acc_in_lds(S::tpr, S::vpt, S::v) ? S::tpr * S::vpt * S::v * (int)sizeof(float) : 0;
+        const int lds = wide_row(S::tpr, S::vpt, S::v) ? S::tpr * S::vpt * S::v * (int)sizeof(float) : 0;
         const auto kernel = rms_norm_bwd_row_kernel<TX, TH, S::tpr, S::vpt, S::v>;
         if (lds > 0) status = odw_set_max_lds(reinterpret_cast<const void*>(kernel), lds);
         if (status != hipSuccess) return;

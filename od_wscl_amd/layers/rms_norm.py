@@ -47,19 +47,29 @@ def _types(x, residual, weight):
     return _BF16[x.dtype] + 2 * _BF16[h.dtype] + (4 * _BF16[weight.dtype] if weight is not None else 0)
 
 
-def _forward(x, weight, residual, eps, want_rstd):
+def _run(what, x, weight, residual, eps, out, rstd=None, scale=None):
+    """The forward launch into `out` (y, or with `scale` the 8-bit codes); returns h (None without a residual)."""
     D = x.shape[-1]
     x2 = _rows(x, D)
     r2 = _rows(residual, D) if residual is not None else None
     w = weight.contiguous() if weight is not None else None
-    R = x2.shape[0]
+    h = torch.empty(x.shape, dtype=residual.dtype, device=x.device) if residual is not None else None
+    args = (x2.data_ptr(), x2.stride(0), 0 if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0), 0 if w is None else w.data_ptr(),
+            x2.shape[0], D, eps, out.data_ptr())
+    hp, types = 0 if h is None else h.data_ptr(), _types(x, residual, weight)
+    if scale is None:
+        code = L.lib().odw_rms_norm(*args, hp, 0 if rstd is None else rstd.data_ptr(), types, L.stream())
+    else:
+        code = L.lib().odw_rms_norm_fp8(*args, scale.data_ptr(), hp, types, L.stream())
+    L.check(code, what)
+    return h
+
+
+def _forward(x, weight, residual, eps, want_rstd):
     with L.on_device_of(x):
-        y = torch.empty((R, D), dtype=x.dtype, device=x.device)
-        h = torch.empty((R, D), dtype=residual.dtype, device=x.device) if residual is not None else None
-        rstd = torch.empty(R, dtype=torch.float32, device=x.device) if want_rstd else None
-        L.check(L.lib().odw_rms_norm(L.ptr(x2), x2.stride(0), L.ptr(r2), r2.stride(0) if r2 is not None else 0, L.ptr(w), R, D, eps, L.ptr(y),
-                                     L.ptr(h), L.ptr(rstd), _types(x, residual, weight), L.stream()), "rms_norm")
-    return y.view(x.shape), h.view(x.shape) if h is not None else None, rstd
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        rstd = torch.empty(x.numel() // x.shape[-1], dtype=torch.float32, device=x.device) if want_rstd else None
+        return y, _run("rms_norm", x, weight, residual, eps, y, rstd=rstd), rstd
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -88,19 +98,16 @@ class _RMSNorm(torch.autograd.Function):
         lib = L.lib()
         with L.on_device_of(h):
             mixed = h_type is not None and h_type != x_type
-            dx = torch.empty((R, D), dtype=x_type, device=h.device) if need_x or (need_r and not mixed) else None
-            dres = torch.empty((R, D), dtype=h_type, device=h.device) if need_r and mixed else None
+            dx = torch.empty(shape, dtype=x_type, device=h.device) if need_x or (need_r and not mixed) else None
+            dres = torch.empty(shape, dtype=h_type, device=h.device) if need_r and mixed else None
             dw = torch.empty_like(w) if need_w else None
             nbytes = lib.odw_rms_norm_bwd_workspace(R, D) if need_w else 0
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device) if need_w else None
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device) if nbytes else None
             types = _BF16[x_type] + 2 * _BF16[x_type if h_type is None else h_type] + (4 * _BF16[w.dtype] if w is not None else 0)
-            L.check(lib.odw_rms_norm_bwd(L.ptr(g2), g2.stride(0), L.ptr(d2), d2.stride(0) if d2 is not None else 0, L.ptr(h2), h2.stride(0),
-                                         L.ptr(w), L.ptr(rstd), R, D, L.ptr(dx), L.ptr(dres), L.ptr(dw), types, L.ptr(ws), nbytes,
-                                         L.stream()), "rms_norm_bwd")
-        dx = dx.view(shape) if dx is not None else None
-        if need_r:
-            dres = dres.view(shape) if mixed else dx
-        return dx if need_x else None, dw, dres if need_r else None, None
+            at = [0 if t is None else t.data_ptr() for t in (g2, d2, h2, w, rstd, dx, dres, dw, ws)]
+            L.check(lib.odw_rms_norm_bwd(at[0], g2.stride(0), at[1], 0 if d2 is None else d2.stride(0), at[2], h2.stride(0), at[3], at[4], R, D,
+                                         at[5], at[6], at[7], types, at[8], nbytes, L.stream()), "rms_norm_bwd")
+        return dx if need_x else None, dw, (dres if mixed else dx) if need_r else None, None
 
 
 def rms_norm(x, weight=None, residual=None, eps=1e-6):
@@ -122,19 +129,11 @@ def rms_norm_fp8(x, weight=None, residual=None, eps=1e-6):
     y ~ q.float() * scale[..., None], scale = max |y| / 448 of the row (2^-126 for a row of zeros); rounded to nearest even.  A row that
     holds a NaN is all NaN.  No gradients."""
     _check("rms_norm_fp8", x, weight, residual, eps)
-    D = x.shape[-1]
-    x2 = _rows(x, D)
-    r2 = _rows(residual, D) if residual is not None else None
-    w = weight.contiguous() if weight is not None else None
-    R = x2.shape[0]
     with L.on_device_of(x):
-        q = torch.empty((R, D), dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty(R, dtype=torch.float32, device=x.device)
-        h = torch.empty((R, D), dtype=residual.dtype, device=x.device) if residual is not None else None
-        L.check(L.lib().odw_rms_norm_fp8(L.ptr(x2), x2.stride(0), L.ptr(r2), r2.stride(0) if r2 is not None else 0, L.ptr(w), R, D, eps, L.ptr(q),
-                                         L.ptr(scale), L.ptr(h), _types(x, residual, weight), L.stream()), "rms_norm_fp8")
-    out = (q.view(x.shape), scale.view(x.shape[:-1]))
-    return out if h is None else out + (h.view(x.shape),)
+        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        h = _run("rms_norm_fp8", x, weight, residual, eps, q, scale=scale)
+    return (q, scale) if h is None else (q, scale, h)
 
 
 class RMSNorm(nn.Module):

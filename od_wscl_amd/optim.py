@@ -12,7 +12,7 @@ the second in float8_e5m2, a power-of-two scale each for every 256 consecutive e
 counter-based stream of utils/rng.py -- a step is a function of its inputs and its key, whatever the launch geometry.
 
 Every tensor is on one GPU; the work goes to the current stream of that device; nothing is read back to the host."""
-import ctypes
+import array
 import math
 
 import torch
@@ -24,31 +24,31 @@ BLOCK = 256          # elements that share a scale of the 8-bit states
 # a gradient whose square is nothing in fp32 (below 1e-21) then moves p by at most lr * 1e-6, not by lr * g / eps of any size
 MIN_EPS = 1e-15
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
+_FLOATS, _F32, _BF16 = {torch.float32, torch.bfloat16}, {torch.float32}, {torch.bfloat16}
+_M8, _V8, _BYTES = {torch.float8_e4m3fn}, {torch.float8_e5m2}, {torch.uint8}
 
 
-def _check_list(what, name, tensors, like, dtypes, blocks=False):
-    """`tensors` beside `like`: as many, on the same GPU, contiguous, of one of `dtypes` and of matching size (`blocks`: two bytes for every
-    256 elements).  Returns their addresses."""
-    if len(tensors) != len(like):
-        raise ValueError("%s: %d %s for %d tensors" % (what, len(tensors), name, len(like)))
-    device = like[0].get_device()
-    at = []
-    for t, p in zip(tensors, like):
-        n = p.numel()
-        if blocks:
-            n = 2 * (-(-n // BLOCK))
-        if t.get_device() != device or t.dtype not in dtypes or t.numel() != n or not t.is_contiguous():
-            i = len(at)
-            L.need_gpu(t)
-            if t.get_device() != device:
-                raise ValueError("%s: %s[%d] is on %s, tensor 0 on %s" % (what, name, i, t.device, like[0].device))
-            if t.dtype not in dtypes:
-                raise TypeError("%s: %s[%d] is %s (%s)" % (what, name, i, t.dtype, " | ".join(str(d) for d in dtypes)))
-            if t.numel() != n:
-                raise ValueError("%s: %s[%d] has %d elements, %d wanted" % (what, name, i, t.numel(), n))
+_numel, _device, _address, _dense = torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+
+
+def _check_list(what, name, tensors, device, sizes, dtypes):
+    """`tensors` beside the first list: as many, on the same GPU, contiguous, of one of `dtypes` and of `sizes`; returns their addresses.
+    (Checked list by list: a call over a hundred tensors costs the host a third of one that looks at each by itself.)"""
+    if (list(map(_numel, tensors)) == sizes and set(map(_device, tensors)) == {device} and {t.dtype for t in tensors} <= dtypes
+            and all(map(_dense, tensors))):
+        return list(map(_address, tensors))
+    if len(tensors) != len(sizes):
+        raise ValueError("%s: %d %s for %d tensors" % (what, len(tensors), name, len(sizes)))
+    L.need_gpu(*tensors)
+    for i, (t, n) in enumerate(zip(tensors, sizes)):
+        if t.get_device() != device:
+            raise ValueError("%s: %s[%d] is on %s, tensor 0 on cuda:%d" % (what, name, i, t.device, device))
+        if t.dtype not in dtypes:
+            raise TypeError("%s: %s[%d] is %s (%s)" % (what, name, i, t.dtype, " | ".join(str(d) for d in dtypes)))
+        if t.numel() != n:
+            raise ValueError("%s: %s[%d] has %d elements, %d wanted" % (what, name, i, t.numel(), n))
+        if not t.is_contiguous():
             raise ValueError("%s: %s[%d] is not contiguous" % (what, name, i))
-        at.append(t.data_ptr())
-    return at
 
 
 def _distinct(what, name, at):
@@ -60,28 +60,32 @@ def _distinct(what, name, at):
             raise ValueError("%s: the same tensor is in `%s` twice" % (what, name))
 
 
-def _ptrs(at):
-    return (ctypes.c_void_p * len(at))(*at)
+class _Lists(object):
+    """Host arrays for a call of the library, alive until it returns (it reads them before that)."""
 
+    def __init__(self):
+        self.kept = []
 
-def _sizes(tensors):
-    return (ctypes.c_int64 * len(tensors))(*[t.numel() for t in tensors])
+    def __call__(self, code, values):
+        a = array.array(code, values)
+        self.kept.append(a)
+        return a.buffer_info()[0] or None
 
 
 def _scalar_list(what, name, value, n):
     if isinstance(value, (int, float)):
-        value = [value] * n
+        value = (value,) * n
     if len(value) != n:
         raise ValueError("%s: %d values of %s for %d tensors" % (what, len(value), name, n))
-    for x in value:
+    for x in set(value):
         if not (x >= 0.0 and math.isfinite(x)):
             raise ValueError("%s: %s = %r" % (what, name, x))
-    return (ctypes.c_float * n)(*value)
+    return value
 
 
 def _device_scalar(what, name, t, device, dtype):
-    if t.numel() != 1 or t.dtype != dtype or t.device != device:
-        raise ValueError("%s: %s has to be one %s on %s (got %s of %d elements on %s)" % (what, name, dtype, device, t.dtype, t.numel(), t.device))
+    if t.numel() != 1 or t.dtype != dtype or t.get_device() != device:
+        raise ValueError("%s: %s has to be one %s on cuda:%d (got %s of %d elements on %s)" % (what, name, dtype, device, t.dtype, t.numel(), t.device))
 
 
 def _grads_of(what, items):
@@ -103,20 +107,21 @@ def _norm(what, grads, max_norm, written=False):
     if not grads:
         raise ValueError("%s: no gradients" % what)
     L.need_gpu(grads[0])
-    at = _check_list(what, "grads", grads, grads, (torch.float32, torch.bfloat16))
+    sizes = list(map(_numel, grads))
+    at = _check_list(what, "grads", grads, grads[0].get_device(), sizes, _FLOATS)
     if written:
         _distinct(what, "grads", at)
     if not max_norm > 0.0:
         raise ValueError("%s: max_norm = %r" % (what, max_norm))
-    lib, n, ptrs = L.lib(), _sizes(grads), _ptrs(at)
-    types = (ctypes.c_int * len(grads))(*[2 * _TYPES[g.dtype] for g in grads])
+    lib, lists, count = L.lib(), _Lists(), len(grads)
+    head = (count, lists("Q", at), lists("q", sizes), lists("i", [2 * _TYPES[g.dtype] for g in grads]))
     with L.on_device_of(grads[0]):
-        nbytes = lib.odw_grad_norm_workspace(len(grads), n)
+        nbytes = lib.odw_grad_norm_workspace(count, head[2])
         ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device) if nbytes else None
         out = torch.empty(2, dtype=torch.float32, device=grads[0].device)
-        L.check(lib.odw_grad_norm(len(grads), ptrs, n, types, float(max_norm), L.ptr(out), L.ptr(ws), nbytes, L.stream()), "grad_norm")
+        L.check(lib.odw_grad_norm(*head, max_norm, L.ptr(out), L.ptr(ws), nbytes, L.stream()), "grad_norm")
         if written:
-            L.check(lib.odw_scale_tensors(len(grads), ptrs, n, types, ctypes.c_void_p(out.data_ptr() + 4), L.stream()), "scale_tensors")
+            L.check(lib.odw_scale_tensors(*head, out.data_ptr() + 4, L.stream()), "scale_tensors")
     return out
 
 
@@ -127,7 +132,7 @@ def grad_norm(grads, max_norm=None):
     that clips them, for `grad_scale` of adamw_step (clipping without a pass over the gradients).  Neither is read by the host.
     A non-finite gradient makes the norm inf or NaN, and coef 0 or NaN."""
     grads = [g if g.is_contiguous() else g.contiguous() for g in _grads_of("grad_norm", grads)]
-    out = _norm("grad_norm", grads, math.inf if max_norm is None else max_norm)
+    out = _norm("grad_norm", grads, math.inf if max_norm is None else float(max_norm))
     return out[0] if max_norm is None else (out[0], out[1])
 
 
@@ -136,7 +141,7 @@ def clip_grad_norm_(grads, max_norm):
     """Scale all of `grads` (tensors, or parameters that stand for their .grad) in place so that their common 2-norm is at most
     max_norm; returns the norm before that (torch.nn.utils.clip_grad_norm_, without a host read)."""
     grads = _grads_of("clip_grad_norm_", grads)
-    out = _norm("clip_grad_norm_", grads, max_norm, written=True)
+    out = _norm("clip_grad_norm_", grads, float(max_norm), written=True)
     torch.autograd.graph.increment_version(grads)
     return out[0]
 
@@ -146,26 +151,26 @@ def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_
     if not params:
         return
     L.need_gpu(params[0])
-    floats = (torch.float32, torch.bfloat16)
-    ap, ag = _check_list(what, "params", params, params, floats), _check_list(what, "grads", grads, params, floats)
-    am = _check_list(what, "exp_avgs", m, params, (torch.float8_e4m3fn,) if bits8 else (torch.float32,))
-    av = _check_list(what, "exp_avg_sqs", v, params, (torch.float8_e5m2,) if bits8 else (torch.float32,))
+    count, device, sizes = len(params), params[0].get_device(), list(map(_numel, params))
+    ap, ag = _check_list(what, "params", params, device, sizes, _FLOATS), _check_list(what, "grads", grads, device, sizes, _FLOATS)
+    am = _check_list(what, "exp_avgs", m, device, sizes, _M8 if bits8 else _F32)
+    av = _check_list(what, "exp_avg_sqs", v, device, sizes, _V8 if bits8 else _F32)
     written = [("params", params, ap), ("exp_avgs", m, am), ("exp_avg_sqs", v, av)]
     if bits8:
-        ae = _check_list(what, "scales", scales, params, (torch.uint8,), blocks=True)
+        ae = _check_list(what, "scales", scales, device, [2 * (-(-n // BLOCK)) for n in sizes], _BYTES)
         written.append(("scales", scales, ae))
     ac = None
     if copies is not None:
-        if len(copies) != len(params):
-            raise ValueError("%s: %d copies for %d tensors" % (what, len(copies), len(params)))
-        have = [(c, p) for c, p in zip(copies, params) if c is not None]
-        at = _check_list(what, "copies", [c for c, _ in have], [p for _, p in have], (torch.bfloat16,)) if have else []
-        written.append(("copies", [c for c, _ in have], at))
-        at = iter(at)
-        ac = [0 if c is None else next(at) for c in copies]
+        if len(copies) != count:
+            raise ValueError("%s: %d copies for %d tensors" % (what, len(copies), count))
+        have = [c for c in copies if c is not None]
+        if have:
+            at = _check_list(what, "copies", have, device, [n for n, c in zip(sizes, copies) if c is not None], _BF16)
+            written.append(("copies", have, at))
+            at = iter(at)
+            ac = [0 if c is None else next(at) for c in copies]
     for name, _, at in written:
         _distinct(what, name, at)
-    count, device = len(params), params[0].device
     if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
         raise ValueError("%s: betas = %r" % (what, betas))
     if not (eps >= MIN_EPS and math.isfinite(eps)):
@@ -175,12 +180,11 @@ def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_
     lr, weight_decay = _scalar_list(what, "lr", lr, count), _scalar_list(what, "weight_decay", weight_decay, count)
     if grad_scale is not None:
         _device_scalar(what, "grad_scale", grad_scale, device, torch.float32)
-    types = (ctypes.c_int * count)(*[_TYPES[p.dtype] + 2 * _TYPES[g.dtype] for p, g in zip(params, grads)])
-    lib, bias = L.lib(), None
+    lib, bias, lists = L.lib(), None, _Lists()
     with L.on_device_of(params[0]):
         if torch.is_tensor(step):
             _device_scalar(what, "step", step, device, torch.int64)
-            bias = torch.empty(4, dtype=torch.float32, device=device)
+            bias = torch.empty(4, dtype=torch.float32, device=params[0].device)
             L.check(lib.odw_adamw_advance(L.ptr(step), betas[0], betas[1], L.ptr(bias), L.stream()), "adamw_advance")
             torch.autograd.graph.increment_version([step])
             number = 0
@@ -190,11 +194,12 @@ def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_
                 raise ValueError("%s: step = %r (the first one is 1)" % (what, step))
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("%s: a captured step would replay step %d for ever: pass `step` as an int64 tensor on the GPU" % (what, number))
-        tail = (_ptrs(ac) if ac is not None else None, _sizes(params), types, lr, weight_decay, betas[0], betas[1], eps, number,
-                L.ptr(bias), L.ptr(grad_scale), grad_mult)
-        head = (count, _ptrs(ap), _ptrs(ag), _ptrs(am), _ptrs(av))
+        head = (count, lists("Q", ap), lists("Q", ag), lists("Q", am), lists("Q", av))
+        tail = (lists("Q", ac) if ac is not None else None, lists("q", sizes),
+                lists("i", [_TYPES[p.dtype] + 2 * _TYPES[g.dtype] for p, g in zip(params, grads)]), lists("f", lr), lists("f", weight_decay),
+                betas[0], betas[1], eps, number, L.ptr(bias), L.ptr(grad_scale), grad_mult)
         if bits8:
-            L.check(lib.odw_adamw8(*head, _ptrs(ae), *tail, key[0], key[1], max_workgroups, L.stream()), what)
+            L.check(lib.odw_adamw8(*head, lists("Q", ae), *tail, key[0], key[1], max_workgroups, L.stream()), what)
         else:
             L.check(lib.odw_adamw(*head, *tail, max_workgroups, L.stream()), what)
     for _, tensors, _ in written:
