@@ -2,7 +2,7 @@
 // global gradient norm it is clipped by.
 //
 // A launch takes up to kMaxTensors tensors: their pointers and sizes travel in the kernel's arguments (no table in device
-// memory to upload, nothing to keep alive for a captured launch).  The tensors are cut into chunks of kChunk elements; a
+// memory to upload, nothing to keep alive for a captured launch).  The tensors are cut into chunks; a
 // workgroup finds the tensor of its chunk by bisection over the chunks' prefix -- the index is uniform, so this is scalar work.
 #include "odw_common.h"
 #include "odw_rng.h"
@@ -11,8 +11,13 @@
 namespace {
 
 constexpr int kMaxTensors = 44;          // (88 B each: the arguments stay under 4 KB)
-constexpr int kChunk = 4096;             // elements a workgroup handles at a time; a multiple of kBlock
 constexpr int kBlock = 256;              // elements that share a scale: one wave, four elements a lane
+// A workgroup's four waves have a whole chunk's loads in flight: 4 blocks a wave of fp32 states, 2 of 8-bit ones (more registers a
+// block).  153 M parameters with bf16 copies, us: fp32 states 825 (2 blocks), 796 (4), 819 (8); 8-bit states 493 (1), 468 (2), 475 (4); chunks
+// of several rounds are slower (4096 elements by 2 blocks: 485; 16384: 528), and so are plain loads (522) or plain stores (511) for the
+// nontemporal ones.
+constexpr int unroll(bool bits8) { return bits8 ? 2 : 4; }
+constexpr int chunk_of(bool bits8) { return unroll(bits8) * 4 * kBlock; }
 constexpr int kNormChunk = 16384;        // the same of the norm: fewer partial sums for the workgroup that adds them
 constexpr int kThreads = 256;
 
@@ -265,17 +270,17 @@ __device__ __forceinline__ void update(const Args& a, const Tensor& t, const Ste
     }
 }
 
-constexpr int kUnroll = 2;
-
-// A chunk: its four waves take every fourth block, kUnroll at a time; the tensor's last, short block by itself.
+// A chunk: its four waves take every fourth block, all at once where the chunk is a whole one; the tensor's last, short block by itself.
 template <bool BITS8, bool PBF, bool GBF>
 __device__ __forceinline__ void chunk(const Args& a, const Tensor& t, const Step& s, int64_t begin, int wave, int lane) {
     const int64_t rest = t.n - begin;
+    constexpr int kChunk = chunk_of(BITS8), kUnroll = unroll(BITS8), kWaves = kThreads / 64;
     const int size = rest < kChunk ? (int)rest : kChunk, blocks = size / kBlock;
-    constexpr int kWaves = kThreads / 64;
     int b = wave;
-    for (; b + (kUnroll - 1) * kWaves < blocks; b += kUnroll * kWaves)
+    if (blocks == kUnroll * kWaves) {
         update<BITS8, PBF, GBF, true, kUnroll>(a, t, s, begin + b * kBlock, kWaves * kBlock, lane, kBlock);
+        return;
+    }
     for (; b < blocks; b += kWaves) update<BITS8, PBF, GBF, true, 1>(a, t, s, begin + b * kBlock, 0, lane, kBlock);
     if (b == blocks && size % kBlock) update<BITS8, PBF, GBF, false, 1>(a, t, s, begin + b * kBlock, 0, lane, size % kBlock);
 }
@@ -296,7 +301,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Args a) {
     for (int c = blockIdx.x; c < a.chunks; c += gridDim.x) {
         const int ti = find_tensor([&](int i) { return a.t[i].chunk0; }, a.count, c);
         const Tensor& t = a.t[ti];
-        const int64_t begin = (int64_t)(c - t.chunk0) * kChunk;
+        const int64_t begin = (int64_t)(c - t.chunk0) * chunk_of(BITS8);
         s.step = t.lr / c1;
         s.decay = t.lr * t.wd;
         switch (t.flags) {                         // (a tensor's types: uniform)
@@ -481,14 +486,14 @@ int adamw(bool bits8, int n_tensors, void* const* p, const void* const* g, void*
         a.count = a.chunks = 0;
         for (; i < n_tensors && a.count < kMaxTensors; ++i) {
             if (n[i] == 0) continue;
-            if (a.count && a.chunks + chunks_of(n[i], kChunk) > INT32_MAX) break;
+            if (a.count && a.chunks + chunks_of(n[i], chunk_of(bits8)) > INT32_MAX) break;
             Tensor& t = a.t[a.count++];
             t.p = p[i]; t.g = g[i]; t.m = m[i]; t.v = v[i]; t.e = bits8 ? e[i] : nullptr;
             t.copy = copy ? (unsigned short*)copy[i] : nullptr;
             t.n = n[i]; t.first = first; t.lr = lr[i]; t.wd = wd[i];
             t.flags = types[i];
             t.chunk0 = a.chunks;
-            a.chunks += (int)chunks_of(n[i], kChunk);
+            a.chunks += (int)chunks_of(n[i], chunk_of(bits8));
             first += (uint64_t)n[i];
         }
         if (!a.count) break;

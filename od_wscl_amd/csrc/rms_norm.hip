@@ -147,7 +147,7 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x, float* part) {
 }
 
 template <class TX, class TH, int TPR, int VPT, int V>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_row_kernel(const TX* __restrict__ x, int64_t ldx, const TH* __restrict__ res,
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1) void rms_norm_row_kernel(const TX* __restrict__ x, int64_t ldx, const TH* __restrict__ res,
                                                                              int64_t ldr, const void* __restrict__ w, int64_t R, int D, float eps,
                                                                              void* __restrict__ y, TH* __restrict__ h, float* __restrict__ rstd,
                                                                              float* __restrict__ scale, int types) {
@@ -441,7 +441,7 @@ template <class... S> struct Shapes {};
 // Rows by width, the first that holds one: a wave a row while a lane needs up to four vectors (no barrier), then 256 and 1024 threads.  The
 // backward pass keeps three numbers an element (gradient, h, the weight's gradient) instead of one: fewer elements a thread.
 typedef Shapes<Shape<64, 1, 4>, Shape<64, 2, 4>, Shape<64, 4, 4>, Shape<256, 2, 4>, Shape<256, 4, 4>, Shape<256, 8, 4>, Shape<1024, 4, 4>,
-               Shape<1024, 8, 4>> Fwd4;
+               Shape<1024, 5, 4>, Shape<1024, 6, 4>, Shape<1024, 7, 4>, Shape<1024, 8, 4>> Fwd4;
 typedef Shapes<Shape<64, 1, 8>, Shape<64, 2, 8>, Shape<64, 4, 8>, Shape<256, 2, 8>, Shape<256, 4, 8>, Shape<256, 8, 8>, Shape<1024, 4, 8>> Fwd8;
 typedef Shapes<Shape<64, 1, 4>, Shape<64, 2, 4>, Shape<64, 4, 4>, Shape<256, 2, 4>, Shape<256, 4, 4>, Shape<1024, 2, 4>, Shape<1024, 4, 4>,
                Shape<1024, 8, 4>> Bwd4;

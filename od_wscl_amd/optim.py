@@ -29,12 +29,13 @@ _M8, _V8, _BYTES = {torch.float8_e4m3fn}, {torch.float8_e5m2}, {torch.uint8}
 
 
 _numel, _device, _address, _dense = torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+_dtype = torch.Tensor.dtype.__get__
 
 
 def _check_list(what, name, tensors, device, sizes, dtypes):
     """`tensors` beside the first list: as many, on the same GPU, contiguous, of one of `dtypes` and of `sizes`; returns their addresses.
     (Checked list by list: a call over a hundred tensors costs the host a third of one that looks at each by itself.)"""
-    if (list(map(_numel, tensors)) == sizes and set(map(_device, tensors)) == {device} and {t.dtype for t in tensors} <= dtypes
+    if (list(map(_numel, tensors)) == sizes and set(map(_device, tensors)) == {device} and set(map(_dtype, tensors)) <= dtypes
             and all(map(_dense, tensors))):
         return list(map(_address, tensors))
     if len(tensors) != len(sizes):
@@ -58,6 +59,11 @@ def _distinct(what, name, at):
         seen.discard(0)
         if len(seen) != len(at) - at.count(0):
             raise ValueError("%s: the same tensor is in `%s` twice" % (what, name))
+
+
+def _types(tensors):
+    kinds = set(map(_dtype, tensors))
+    return [_TYPES[kinds.pop()]] * len(tensors) if len(kinds) == 1 else [_TYPES[t.dtype] for t in tensors]
 
 
 class _Lists(object):
@@ -114,7 +120,7 @@ def _norm(what, grads, max_norm, written=False):
     if not max_norm > 0.0:
         raise ValueError("%s: max_norm = %r" % (what, max_norm))
     lib, lists, count = L.lib(), _Lists(), len(grads)
-    head = (count, lists("Q", at), lists("q", sizes), lists("i", [2 * _TYPES[g.dtype] for g in grads]))
+    head = (count, lists("Q", at), lists("q", sizes), lists("i", [2 * t for t in _types(grads)]))
     with L.on_device_of(grads[0]):
         nbytes = lib.odw_grad_norm_workspace(count, head[2])
         ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device) if nbytes else None
@@ -196,7 +202,7 @@ def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_
                 raise RuntimeError("%s: a captured step would replay step %d for ever: pass `step` as an int64 tensor on the GPU" % (what, number))
         head = (count, lists("Q", ap), lists("Q", ag), lists("Q", am), lists("Q", av))
         tail = (lists("Q", ac) if ac is not None else None, lists("q", sizes),
-                lists("i", [_TYPES[p.dtype] + 2 * _TYPES[g.dtype] for p, g in zip(params, grads)]), lists("f", lr), lists("f", weight_decay),
+                lists("i", [tp + 2 * tg for tp, tg in zip(_types(params), _types(grads))]), lists("f", lr), lists("f", weight_decay),
                 betas[0], betas[1], eps, number, L.ptr(bias), L.ptr(grad_scale), grad_mult)
         if bits8:
             L.check(lib.odw_adamw8(*head, lists("Q", ae), *tail, key[0], key[1], max_workgroups, L.stream()), what)
