@@ -126,6 +126,13 @@ def make_defaults():
     # stacked views' operand is allocated for twice that many rows (150 KB each at VGG16 / 7 x 7); a step that samples more
     # raises (loudly, one or two steps later)
     c.ODW.MAX_SAMPLED_ROWS = 4096
+    # the optimiser (engine.build_optimizer): "SGD" (the reference's, SOLVER.MOMENTUM) or "ADAMW" with these betas and eps, its two
+    # averages in 32 or 8 bits, and -- CLIP_NORM > 0 -- the gradient's global norm clipped to that
+    c.ODW.OPTIMIZER = "SGD"
+    c.ODW.ADAM_BETAS = (0.9, 0.999)
+    c.ODW.ADAM_EPS = 1e-8
+    c.ODW.STATE_BITS = 32
+    c.ODW.CLIP_NORM = 0.0
     c.SEED = -1
     c.min_size = 20                                           # :550
     return c

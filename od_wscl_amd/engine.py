@@ -225,7 +225,6 @@ class FlatSGD(object):
         dev = order[0][1].device
         self.flat_p = torch.empty(total, dtype=torch.float32, device=dev)
         self.flat_g = torch.zeros(total, dtype=torch.float32, device=dev)
-        self.flat_m = torch.zeros(total, dtype=torch.float32, device=dev)
         off = 0
         self.slices = {}
         for (n, p), sz in zip(order, sizes):
@@ -244,6 +243,7 @@ class FlatSGD(object):
              cfg.SOLVER.WEIGHT_DECAY_BIAS)]
         self.gemm_params = [p for _, p in gemm_w]
         self.n_gemm = n_gemm
+        self._make_state(total, dev)
         # (ODW_PRIO = "step,optimiser,contrastive" stream priorities, an experiment knob.  Default 0,0,0 since the end of round 6:
         # EVERY stream of the process at normal priority, so that all of them share the runtime's pool of GPU_MAX_HW_QUEUES = 4
         # hardware queues.  A stream of another priority gets a queue of its own, and with five queues busy at once the whole
@@ -326,6 +326,9 @@ class FlatSGD(object):
                 pred.set_fused(w_cat, b_cat, managed_shadow(w_cat, ow))
                 self.gemm_params.append(w_cat)
             self._refresh_shadows(initial=True)
+
+    def _make_state(self, total, device):
+        self.flat_m = torch.zeros(total, dtype=torch.float32, device=device)
 
     def _refresh_shadows(self, initial=False):
         from . import gemm
@@ -463,6 +466,11 @@ class FlatSGD(object):
         self.hold = False
         self.exchange.begin()
 
+    def _update(self, regions, paced=0):
+        """The fused update of some of the regions, on the current stream."""
+        for i in regions:
+            self._sgd_region(i, paced)
+
     def _sgd_region(self, i, paced=0):
         """paced = workgroup cap of an update that runs BESIDE other kernels (head_grads_ready): at full width the
         HBM-bound pass starves whatever shares the GPU with it (the first backbone weight-gradient GEMM took 400 us
@@ -493,7 +501,7 @@ class FlatSGD(object):
         with torch.cuda.stream(self.side):
             self.exchange.finish(0, self.n_gemm)       # what the weight-gradient GEMMs did not hand over as they retired
             # (paced only without an exchange in front of it: at N > 1 the all-reduce already takes the window)
-            self._sgd_region(0, paced=int(os.environ.get("ODW_SGD_PACE", "160")) if self.world == 1 else 0)
+            self._update((0,), paced=int(os.environ.get("ODW_SGD_PACE", "160")) if self.world == 1 else 0)
             self._refresh_shadows()
         self.early_done = True
 
@@ -521,10 +529,9 @@ class FlatSGD(object):
     def step(self):
         self.flush_wgrad()
         if not self.early_done:
-            self._sgd_region(0)
+            self._update((0,))
             self._refresh_shadows()
-        self._sgd_region(1)
-        self._sgd_region(2)
+        self._update((1, 2))
         if self.early_done:
             # the next forward reads the refreshed weights -- but not before its first head GEMM, ~2 ms of backbone
             # forward away: the wait is handed to the shadows (gemm.Shadow.refresh) instead of blocking the stream here.
@@ -547,6 +554,150 @@ class FlatSGD(object):
             self._head_event = None
             for sh in self.shadows:
                 sh.pending = None
+
+
+class FlatAdamW(FlatSGD):
+    """AdamW over FlatSGD's flat buffers (ODW.OPTIMIZER "ADAMW"; decoupled decay with SOLVER.WEIGHT_DECAY / WEIGHT_DECAY_BIAS, learning rates
+    and schedule as for SGD, no momentum correction).  Same orchestration: the head's region on the side stream as soon as its gradients
+    are final, the bf16 shadow rewritten in the same pass, the exchange's 1/world folded in.
+
+    ODW.STATE_BITS 32, or 8: the averages as 8-bit floats with block scales (optim.adamw8_step), 2 bytes a parameter instead of 8 --
+    0.3 GB instead of 1.2 for VGG16/VOC.  ODW.CLIP_NORM > 0 clips the averaged gradient's global norm: every gradient has to be
+    there before anything is updated, so the head's update then waits for the end of the backward."""
+
+    def __init__(self, cfg, model, world=1):
+        odw = cfg.ODW
+        self.bits, self.betas, self.eps = int(odw.STATE_BITS), tuple(odw.ADAM_BETAS), float(odw.ADAM_EPS)
+        self.clip_norm = float(odw.CLIP_NORM)
+        if self.bits not in (8, 32):
+            raise ValueError("ODW.STATE_BITS = %r (8 | 32)" % (odw.STATE_BITS,))
+        if not self.clip_norm >= 0.0:
+            raise ValueError("ODW.CLIP_NORM = %r" % (odw.CLIP_NORM,))
+        self.steps = 0                  # updates taken
+        self.grad_norm = None           # of the last step, where it was clipped (0-dim, on the GPU)
+        super().__init__(cfg, model, world)
+
+    def _make_state(self, total, device):
+        from . import optim
+        if self.bits == 8:
+            # (a block of 256 elements must not straddle regions, which are updated apart: states region by region)
+            self.state8 = [optim.state8_zeros(self.flat_p[s:s + n]) for s, n, _, _ in self.regions]
+        else:
+            self.flat_m = torch.zeros(total, dtype=torch.float32, device=device)
+            self.flat_v = torch.zeros(total, dtype=torch.float32, device=device)
+
+    def _update(self, regions, paced=0):
+        from . import optim
+        from .utils import rng
+        if self.clip_norm > 0.0 and 0 in regions:
+            # (the norm of the mean over the ranks is the sum's over world)
+            norm, self._coef = optim.grad_norm([self.flat_g], max_norm=self.clip_norm * self.world)
+            self.grad_norm = norm / self.world
+        which = [i for i in regions if self.regions[i][1] > 0]
+        cut = [self.regions[i] for i in which]
+        p, g = ([flat[s:s + n] for s, n, _, _ in cut] for flat in (self.flat_p, self.flat_g))
+        copies = [self.flat_w16 if i == 0 else None for i in which]
+        more = dict(lr=[lr * self.lr_scale for _, _, lr, _ in cut], weight_decay=[wd for _, _, _, wd in cut], betas=self.betas, eps=self.eps,
+                    grad_scale=self._coef, copies=copies, grad_mult=1.0 / self.world, max_workgroups=int(paced))
+        if self.bits == 8:
+            m, v, e = ([self.state8[i][k] for i in which] for k in range(3))
+            key = rng.stream_key(self.cfg.SEED & 0xFFFFFFFF, (1 << 40) + 4 * self.steps + regions[0])
+            optim.adamw8_step(p, g, m, v, e, self.steps + 1, key, **more)
+        else:
+            m, v = ([flat[s:s + n] for s, n, _, _ in cut] for flat in (self.flat_m, self.flat_v))
+            optim.adamw_step(p, g, m, v, self.steps + 1, **more)
+
+    _coef = None
+
+    def head_grads_ready(self):
+        if self.clip_norm == 0.0:
+            super().head_grads_ready()
+
+    def all_reduce(self):
+        if self.clip_norm > 0.0:
+            self.flush_wgrad()          # (nothing has flushed the weight-gradient batches early)
+        super().all_reduce()
+
+    def step(self):
+        super().step()
+        self.steps += 1
+
+    def set_iteration(self, iteration):
+        self.lr_scale = lr_factor(self.cfg, iteration)
+
+    # ---- torch.optim.AdamW's layout, one group per trainable parameter like FlatSGD's
+    def _averages(self):
+        """Both averages as flat fp32 buffers (of 8-bit states: exactly what they hold)."""
+        from . import optim
+        if self.bits == 32:
+            return self.flat_m, self.flat_v
+        out = [torch.zeros_like(self.flat_p) for _ in range(2)]
+        for (s, n, _, _), st in zip(self.regions, self.state8):
+            for flat, x in zip(out, optim.state8_read(*st)):
+                flat[s:s + n].copy_(x)
+        return out
+
+    def state_dict(self, model):
+        s = self.cfg.SOLVER
+        self.join_side()
+        groups, state = [], {}
+        m, v = self._averages() if self.steps > 0 else (None, None)
+        shapes = {n: p.shape for n, p in model.named_parameters()}
+        for i, n in enumerate(self._param_order(model)):
+            off, numel = self.slices[n]
+            bias = "bias" in n
+            groups.append({"lr": (s.BASE_LR * s.BIAS_LR_FACTOR if bias else s.BASE_LR) * self.lr_scale, "betas": self.betas, "eps": self.eps,
+                           "weight_decay": s.WEIGHT_DECAY_BIAS if bias else s.WEIGHT_DECAY, "amsgrad": False, "maximize": False,
+                           "foreach": None, "capturable": False, "differentiable": False, "fused": None, "params": [i]})
+            if self.steps > 0:
+                state[i] = {"step": torch.tensor(float(self.steps)), "exp_avg": m[off:off + numel].view(shapes[n]).clone(),
+                            "exp_avg_sq": v[off:off + numel].view(shapes[n]).clone()}
+        return {"state": state, "param_groups": groups}
+
+    def load_state_dict(self, model, sd):
+        """Averages and step count of a checkpoint written by state_dict() above (with either STATE_BITS) or by torch.optim.AdamW."""
+        from . import optim
+        self.join_side()
+        order = self._param_order(model)
+        state = sd.get("state", {})
+        if len(sd.get("param_groups", order)) != len(order):
+            raise ValueError("optimizer state has %d parameter groups, the model %d trainable parameters" % (len(sd["param_groups"]), len(order)))
+        if any("momentum_buffer" in st for st in state.values()):
+            raise ValueError("the checkpoint's optimizer state is SGD's momentum; ODW.OPTIMIZER is ADAMW")
+        flat = [torch.zeros_like(self.flat_p) for _ in range(2)]
+        steps = set()
+        for i, n in enumerate(order):
+            entry = state.get(i, state.get(str(i)))
+            if entry is None:
+                continue
+            off, numel = self.slices[n]
+            for f, k in zip(flat, ("exp_avg", "exp_avg_sq")):
+                f[off:off + numel].copy_(entry[k].reshape(-1).to(f.device))
+            steps.add(int(entry["step"]))
+        if not steps:
+            return 0
+        if len(steps) != 1:
+            raise ValueError("optimizer state: parameters have taken different numbers of steps %s" % sorted(steps))
+        if self.bits == 8:
+            for (s, n, _, _), st in zip(self.regions, self.state8):
+                optim.state8_write(flat[0][s:s + n], flat[1][s:s + n], out=st)
+        else:
+            self.flat_m, self.flat_v = flat
+        self.steps = steps.pop()
+        self.first = False
+        return len(state)
+
+
+def build_optimizer(cfg, model, world=1):
+    """The optimiser over the model's flat buffers (the place of solver/build.py:10-24): ODW.OPTIMIZER "SGD" | "ADAMW"."""
+    kind = cfg.ODW.OPTIMIZER
+    if kind == "ADAMW":
+        return FlatAdamW(cfg, model, world)
+    if kind != "SGD":
+        raise ValueError("ODW.OPTIMIZER = %r (SGD | ADAMW)" % (kind,))
+    if cfg.ODW.CLIP_NORM != 0.0:
+        raise ValueError("ODW.CLIP_NORM needs ODW.OPTIMIZER ADAMW (the reference's SGD does not clip)")
+    return FlatSGD(cfg, model, world)
 
 
 def build_training_step(cfg, device, dtype="bf16", world=1, seed=1234, backend="hip"):
@@ -588,7 +739,7 @@ def build_training_step(cfg, device, dtype="bf16", world=1, seed=1234, backend="
         conv_desc = "od_wscl_amd HIP implicit-GEMM conv3x3 (NHWC, MFMA)"
     else:
         conv_desc = "od_wscl_amd HIP: 1x1 convs on the MFMA GEMM, implicit-GEMM conv3x3, folded frozen BN (NHWC)"
-    opt = FlatSGD(cfg, model, world)
+    opt = build_optimizer(cfg, model, world)
     model.roi_heads.head_grads_ready = opt.head_grads_ready
     # N > 1: the body's backward in three runs of layers (conv5 / conv4 / conv3 for VGG16), each run's weight gradients
     # handed to the exchange when its launches are queued -- on a stream of their own: the side stream is busy with the
@@ -731,5 +882,5 @@ def build_training_step(cfg, device, dtype="bf16", world=1, seed=1234, backend="
     step.model, step.optimizer = model, opt
     mode = precision.get_precision()
     info = {"gemm_backend": "od_wscl_amd HIP MFMA gemm_nt_bf16 (%s operands, fp32 acc)" % mode,
-            "conv_backend": conv_desc + " " + mode, "optimizer": "od_wscl_amd fused flat SGD", "precision": mode}
+            "conv_backend": conv_desc + " " + mode, "optimizer": "od_wscl_amd fused flat " + ("AdamW, %d-bit states" % opt.bits if isinstance(opt, FlatAdamW) else "SGD"), "precision": mode}
     return step, info

@@ -3,7 +3,7 @@
 The reference trains with SGD only (solver/build.py:10-24, engine.FlatSGD here); this is the optimiser beside it, for heads
 that do not train well under SGD.  Three ways in:
 
-  * `SOLVER.OPTIMIZER "ADAMW"`: the training step of engine.build_training_step (tools/train_net.py) runs it over its flat buffers;
+  * `ODW.OPTIMIZER "ADAMW"`: the training step of engine.build_training_step (tools/train_net.py) runs it over its flat buffers;
   * `AdamW`, a torch.optim.Optimizer, for a module of one's own;
   * `adamw_step` / `adamw8_step` / `grad_norm` / `clip_grad_norm_` on lists of tensors.
 
