@@ -11,6 +11,11 @@ namespace {
 
 enum { kXBf16 = 1, kHBf16 = 2, kWBf16 = 4 };
 
+// Outputs of the forward pass over this many bytes (the eight L2s together) are stored past the caches (PAST): nothing of them would be left
+// there for the next kernel, and the rows coming in keep their place.  2000 x 4096 fp32 with residual 27.7 us -> 20.1 (6.5 TB/s),
+// 16000 x 4096 bf16 96 -> 91.  (Loads past the caches: 30 and 106; stores of the backward pass: no difference.)
+constexpr int64_t kL2Bytes = (int64_t)32 << 20;
+
 __device__ __forceinline__ float ld(const void* p, bool bf, int64_t i) {
     return bf ? __uint_as_float((uint32_t)((const unsigned short*)p)[i] << 16) : ((const float*)p)[i];
 }
@@ -86,13 +91,14 @@ __device__ __forceinline__ void load(const T* src, int left, float (&x)[V]) {
 #pragma unroll
     for (int j = 0; j < V; ++j) x[j] = up((T)u[j]);
 }
-template <class T, int V>
+template <class T, int V, bool PAST = false>
 __device__ __forceinline__ void store(T* dst, int left, const float (&x)[V]) {
     if (left >= V) {
         typename Vec<T, V>::full u;
 #pragma unroll
         for (int j = 0; j < V; ++j) u[j] = down<T>(x[j]);
-        *reinterpret_cast<typename Vec<T, V>::t*>(dst) = u;
+        if (PAST) __builtin_nontemporal_store(u, reinterpret_cast<typename Vec<T, V>::t*>(dst));
+        else *reinterpret_cast<typename Vec<T, V>::t*>(dst) = u;
     } else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -146,7 +152,7 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x, float* part) {
     return x;
 }
 
-template <class TX, class TH, int TPR, int VPT, int V>
+template <class TX, class TH, int TPR, int VPT, int V, bool PAST>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1) void rms_norm_row_kernel(const TX* __restrict__ x, int64_t ldx, const TH* __restrict__ res,
                                                                              int64_t ldr, const void* __restrict__ w, int64_t R, int D, float eps,
                                                                              void* __restrict__ y, TH* __restrict__ h, float* __restrict__ rstd,
@@ -179,7 +185,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1) void rms_
                 load<TH, V>(res + r * ldr + i, D - i, a);
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[k][j] = up(down<TH>(v[k][j] + a[j]));
-                store<TH, V>(h + r * D + i, D - i, v[k]);
+                store<TH, V, PAST>(h + r * D + i, D - i, v[k]);
             }
         }
     }
@@ -200,7 +206,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1) void rms_
 #pragma unroll
             for (int j = 0; j < V; ++j) v[k][j] = v[k][j] * rs * g[j];
             if (!scale) {
-                store<TX, V>((TX*)y + r * D + i, D - i, v[k]);
+                store<TX, V, PAST>((TX*)y + r * D + i, D - i, v[k]);
             } else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
@@ -353,22 +359,24 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_row_kernel
     }
 }
 
-// 64 columns a workgroup, the rows of part_w over its 16 waves.
+// 32 columns a workgroup, the rows of part_w over its 32 groups of 32 lanes.
 __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restrict__ part_w, int G, int D, void* __restrict__ dw, int types) {
-    __shared__ float part[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+    constexpr int kCols = 32, kSlices = 1024 / kCols;
+    __shared__ float part[kSlices][kCols + 1];
+    const int c = threadIdx.x % kCols, slice = threadIdx.x / kCols;
+    const int64_t i = (int64_t)blockIdx.x * kCols + c;
     float s = 0.0f;
     if (i < D)
 #pragma unroll 8
-        for (int g = wave; g < G; g += 16) s += part_w[(int64_t)g * D + i];
-    part[wave][lane] = s;
+        for (int g = slice; g < G; g += kSlices) s += part_w[(int64_t)g * D + i];
+    part[slice][c] = s;
     __syncthreads();
-    if (wave == 0 && i < D) {
-#pragma unroll
-        for (int k = 1; k < 16; ++k) s += part[k][lane];
-        st(dw, types & kWBf16, i, s);
+    // the slices' sums by halves, in one order
+    for (int half = kSlices / 2; half > 0; half /= 2) {
+        if (slice < half) part[slice][c] += part[slice + half][c];
+        __syncthreads();
     }
+    if (slice == 0 && i < D) st(dw, types & kWBf16, i, part[0][c]);
 }
 
 // ---- rows of any width: the workgroup walks a row as often as it needs it -------------------------------------------------------
@@ -438,11 +446,14 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(const void* dy, int64
 template <int T_, int K_, int V_> struct Shape { static constexpr int tpr = T_, vpt = K_, v = V_; };
 template <class... S> struct Shapes {};
 
-// Rows by width, the first that holds one: a wave a row while a lane needs up to four vectors (no barrier), then 256 and 1024 threads.  The
-// backward pass keeps three numbers an element (gradient, h, the weight's gradient) instead of one: fewer elements a thread.
-typedef Shapes<Shape<64, 1, 4>, Shape<64, 2, 4>, Shape<64, 4, 4>, Shape<256, 2, 4>, Shape<256, 4, 4>, Shape<256, 8, 4>, Shape<1024, 4, 4>,
+// Rows by width, the first that holds one: a wave a row while a lane needs one or two vectors (no barrier), then 256 and 1024 threads.  16000 x
+// 1024 fp32 with a wave and four vectors a lane 49.1 us, with 256 threads 45.7; 4000 x 8192 bf16 with 256 threads and four vectors 53.7,
+// with 1024 threads 52.0.  1024 threads of up to 64 registers leave room for a second row on a compute unit: 2000 x 25088 fp32 to
+// 8 bits 72 us with one row, 56 with two.  The backward pass keeps three numbers an element (gradient, h, the weight's gradient)
+// instead of one: fewer elements a thread.
+typedef Shapes<Shape<64, 1, 4>, Shape<64, 2, 4>, Shape<256, 1, 4>, Shape<256, 2, 4>, Shape<256, 4, 4>, Shape<256, 8, 4>, Shape<1024, 4, 4>,
                Shape<1024, 5, 4>, Shape<1024, 6, 4>, Shape<1024, 7, 4>, Shape<1024, 8, 4>> Fwd4;
-typedef Shapes<Shape<64, 1, 8>, Shape<64, 2, 8>, Shape<64, 4, 8>, Shape<256, 2, 8>, Shape<256, 4, 8>, Shape<256, 8, 8>, Shape<1024, 4, 8>> Fwd8;
+typedef Shapes<Shape<64, 1, 8>, Shape<64, 2, 8>, Shape<256, 1, 8>, Shape<256, 2, 8>, Shape<1024, 1, 8>, Shape<1024, 2, 8>, Shape<1024, 4, 8>> Fwd8;
 typedef Shapes<Shape<64, 1, 4>, Shape<64, 2, 4>, Shape<64, 4, 4>, Shape<256, 2, 4>, Shape<256, 4, 4>, Shape<1024, 2, 4>, Shape<1024, 4, 4>,
                Shape<1024, 8, 4>> Bwd4;
 typedef Shapes<Shape<64, 1, 8>, Shape<64, 2, 8>, Shape<256, 1, 8>, Shape<256, 2, 8>, Shape<1024, 1, 8>, Shape<1024, 2, 8>, Shape<1024, 4, 8>> Bwd8;
@@ -453,9 +464,12 @@ bool with_shape(int D, Shapes<S...>, F f) {
     return ((D <= S::tpr * S::vpt * S::v ? (f(S()), true) : false) || ...);
 }
 
-// Row groups of the backward pass = rows of part_w: enough to fill the chip, few beside the rows.
+// Row groups of the backward pass = rows of part_w: enough to fill the chip, few beside the rows.  Measured, us: 16000 x 4096 bf16 (256 threads
+// a row) 512 groups 101, 768 107, 1024 123; 40000 x 512 bf16 (a wave a row) 1024 groups 66, 2048 45, 4096 49; 3000 x 128 fp32 1024 groups
+// 10, 2048 13.
 int bwd_groups(int64_t R, int D) {
-    const int most = D <= 1024 ? 1024 : D <= 4096 ? 512 : 256;
+    if (D <= 1024) return (int)(R < 64 ? R : R < 8192 ? (R + 3) / 4 : 2048);        // (waves)
+    const int most = D <= 4096 ? 512 : 256;
     return (int)(R < most ? R : most);
 }
 
@@ -470,10 +484,12 @@ template <class TX, class TH>
 void forward(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, int64_t R, int D, float eps, void* y, void* h, float* rstd,
              float* scale, int types, hipStream_t stream) {
     constexpr int V = sizeof(TX) == 2 ? 8 : 4;
+    const bool past = R * D * (int64_t)((scale ? 1 : sizeof(TX)) + (res ? sizeof(TH) : 0)) > kL2Bytes;
     auto launch = [&](auto s) {
         typedef decltype(s) S;
         constexpr int kRows = S::tpr > 256 ? 1 : 256 / S::tpr;
-        rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v><<<(unsigned)((R + kRows - 1) / kRows), kRows * S::tpr, 0, stream>>>(
+        const auto kernel = past ? rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v, true> : rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v, false>;
+        kernel<<<(unsigned)((R + kRows - 1) / kRows), kRows * S::tpr, 0, stream>>>(
             (const TX*)x, ldx, (const TH*)res, ldr, w, R, D, eps, y, (TH*)h, rstd, scale, types);
     };
     if (R < ((int64_t)1 << 31)) {
@@ -573,7 +589,7 @@ ODW_EXPORT int odw_rms_norm_bwd(const void* dy, int64_t ld_dy, const void* dh, i
         ODW_CHECK_LAUNCH("rms_norm_bwd_kernel");
     }
     if (dw) {
-        rms_norm_dw_kernel<<<(unsigned)(((int64_t)D + 63) / 64), 1024, 0, stream>>>((const float*)workspace, groups, D, dw, types);
+        rms_norm_dw_kernel<<<(unsigned)(((int64_t)D + 31) / 32), 1024, 0, stream>>>((const float*)workspace, groups, D, dw, types);
         ODW_CHECK_LAUNCH("rms_norm_dw_kernel");
     }
     return ODW_OK;
