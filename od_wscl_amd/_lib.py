@@ -237,13 +237,15 @@ def stream():
 
 
 _no_guard = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device_of(t):
     """Context in which the current device is t's (launches go to the current device's current stream); nothing to do in the usual
     case that it is already."""
     index = t.get_device()
-    return _no_guard if index == torch.cuda.current_device() else torch.cuda.device(index)
+    # (t is on a GPU, so the runtime is up: its own query, a tenth of torch.cuda.current_device())
+    return _no_guard if index == _current_device() else torch.cuda.device(index)
 
 
 def ptr(t):

@@ -18,6 +18,7 @@ constexpr int kBlock = 256;              // elements that share a scale: one wav
 // nontemporal ones.
 constexpr int unroll(bool bits8) { return bits8 ? 2 : 4; }
 constexpr int chunk_of(bool bits8) { return unroll(bits8) * 4 * kBlock; }
+constexpr int kMaxGrid = 1 << 23;        // (a launch has fewer than 2^32 threads; the update's workgroups walk on, the norm's chunks are enough)
 constexpr int kNormChunk = 16384;        // the same of the norm: fewer partial sums for the workgroup that adds them
 constexpr int kThreads = 256;
 
@@ -497,7 +498,8 @@ int adamw(bool bits8, int n_tensors, void* const* p, const void* const* g, void*
             first += (uint64_t)n[i];
         }
         if (!a.count) break;
-        const int grid = max_workgroups > 0 && max_workgroups < a.chunks ? max_workgroups : a.chunks;
+        const int most = max_workgroups > 0 && max_workgroups < kMaxGrid ? max_workgroups : kMaxGrid;
+        const int grid = a.chunks < most ? a.chunks : most;
         if (bits8) adamw_kernel<true><<<grid, kThreads, 0, stream>>>(a);
         else adamw_kernel<false><<<grid, kThreads, 0, stream>>>(a);
         ODW_CHECK_LAUNCH("adamw_kernel");

@@ -489,13 +489,18 @@ void forward(const void* x, int64_t ldx, const void* res, int64_t ldr, const voi
         typedef decltype(s) S;
         constexpr int kRows = S::tpr > 256 ? 1 : 256 / S::tpr;
         const auto kernel = past ? rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v, true> : rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v, false>;
-        kernel<<<(unsigned)((R + kRows - 1) / kRows), kRows * S::tpr, 0, stream>>>(
-            (const TX*)x, ldx, (const TH*)res, ldr, w, R, D, eps, y, (TH*)h, rstd, scale, types);
+        // (a launch has fewer than 2^32 threads: rows beyond go to further ones)
+        constexpr int64_t kMost = (int64_t)1 << 21;
+        for (int64_t r = 0; r < R; r += kMost * kRows) {
+            const int64_t n = R - r < kMost * kRows ? R - r : kMost * kRows;
+            kernel<<<(unsigned)((n + kRows - 1) / kRows), kRows * S::tpr, 0, stream>>>(
+                (const TX*)x + r * ldx, ldx, res ? (const TH*)res + r * ldr : nullptr, ldr, w, n, D, eps,
+                (char*)y + r * D * (int64_t)(scale ? 1 : sizeof(TX)), res ? (TH*)h + r * D : nullptr, rstd ? rstd + r : nullptr,
+                scale ? scale + r : nullptr, types);
+        }
     };
-    if (R < ((int64_t)1 << 31)) {
-        if constexpr (V == 8) { if (with_shape(D, Fwd8(), launch)) return; }
-        else { if (with_shape(D, Fwd4(), launch)) return; }
-    }
+    if constexpr (V == 8) { if (with_shape(D, Fwd8(), launch)) return; }
+    else { if (with_shape(D, Fwd4(), launch)) return; }
     const unsigned grid = (unsigned)(R < 65536 ? R : 65536);
     if (scale) rms_norm_kernel<true><<<grid, 256, 0, stream>>>(x, ldx, res, ldr, w, R, D, eps, y, h, rstd, scale, types);
     else rms_norm_kernel<false><<<grid, 256, 0, stream>>>(x, ldx, res, ldr, w, R, D, eps, y, h, rstd, scale, types);

@@ -414,6 +414,8 @@ class FlatSGD(object):
         if len(sd.get("param_groups", order)) != len(order):
             raise ValueError("optimizer state has %d parameter groups, the model %d trainable parameters"
                              % (len(sd["param_groups"]), len(order)))
+        if any("exp_avg" in st for st in state.values()):
+            raise ValueError("the checkpoint's optimizer state is Adam's averages; ODW.OPTIMIZER is SGD")
         loaded = 0
         for i, n in enumerate(order):
             entry = state.get(i, state.get(str(i)))

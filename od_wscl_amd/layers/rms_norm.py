@@ -53,7 +53,7 @@ def _run(what, x, weight, residual, eps, out, rstd=None, scale=None):
     x2 = _rows(x, D)
     r2 = _rows(residual, D) if residual is not None else None
     w = weight.contiguous() if weight is not None else None
-    h = torch.empty(x.shape, dtype=residual.dtype, device=x.device) if residual is not None else None
+    h = residual.new_empty(x.shape) if residual is not None else None
     args = (x2.data_ptr(), x2.stride(0), 0 if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0), 0 if w is None else w.data_ptr(),
             x2.shape[0], D, eps, out.data_ptr())
     hp, types = 0 if h is None else h.data_ptr(), _types(x, residual, weight)
@@ -67,8 +67,8 @@ def _run(what, x, weight, residual, eps, out, rstd=None, scale=None):
 
 def _forward(x, weight, residual, eps, want_rstd):
     with L.on_device_of(x):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        rstd = torch.empty(x.numel() // x.shape[-1], dtype=torch.float32, device=x.device) if want_rstd else None
+        y = x.new_empty(x.shape)
+        rstd = x.new_empty(x.numel() // x.shape[-1], dtype=torch.float32) if want_rstd else None
         return y, _run("rms_norm", x, weight, residual, eps, y, rstd=rstd), rstd
 
 
@@ -82,32 +82,39 @@ class _RMSNorm(torch.autograd.Function):
         return y if h is None else (y, h)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
-        x_type, h_type = ctx.dtypes
-        need_x, need_w, need_r = ctx.needs_input_grad[:3]
-        if dy is None:                                # only h was used
-            return (dh.to(x_type) if need_x and dh is not None else None, None if not need_w else torch.zeros_like(weight),
-                    dh if need_r else None, None)
-        D, shape = h.shape[-1], h.shape
-        h2, g2 = _rows(h, D), _rows(dy, D)
-        d2 = _rows(dh, D) if dh is not None else None
-        w = weight.contiguous() if weight is not None else None
-        R = h2.shape[0]
-        lib = L.lib()
-        with L.on_device_of(h):
-            mixed = h_type is not None and h_type != x_type
-            dx = torch.empty(shape, dtype=x_type, device=h.device) if need_x or (need_r and not mixed) else None
-            dres = torch.empty(shape, dtype=h_type, device=h.device) if need_r and mixed else None
-            dw = torch.empty_like(w) if need_w else None
-            nbytes = lib.odw_rms_norm_bwd_workspace(R, D) if need_w else 0
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device) if nbytes else None
-            types = _BF16[x_type] + 2 * _BF16[x_type if h_type is None else h_type] + (4 * _BF16[w.dtype] if w is not None else 0)
-            at = [0 if t is None else t.data_ptr() for t in (g2, d2, h2, w, rstd, dx, dres, dw, ws)]
-            L.check(lib.odw_rms_norm_bwd(at[0], g2.stride(0), at[1], 0 if d2 is None else d2.stride(0), at[2], h2.stride(0), at[3], at[4], R, D,
-                                         at[5], at[6], at[7], types, at[8], nbytes, L.stream()), "rms_norm_bwd")
-        return dx if need_x else None, dw, (dres if mixed else dx) if need_r else None, None
+        # (once_differentiable's bookkeeping is a third of the host's time here; without create_graph it has nothing to do)
+        return _backward_once(ctx, dy, dh) if torch.is_grad_enabled() else _backward(ctx, dy, dh)
+
+
+def _backward(ctx, dy, dh):
+    h, weight, rstd = ctx.saved_tensors
+    x_type, h_type = ctx.dtypes
+    need_x, need_w, need_r = ctx.needs_input_grad[:3]
+    if dy is None:                                # only h was used
+        return (dh.to(x_type) if need_x and dh is not None else None, torch.zeros_like(weight) if need_w else None, dh if need_r else None, None)
+    shape = h.shape
+    D = shape[-1]
+    h2, g2 = _rows(h, D), _rows(dy, D)
+    d2 = _rows(dh, D) if dh is not None else None
+    w = weight.contiguous() if weight is not None else None
+    R = h2.shape[0]
+    lib = L.lib()
+    with L.on_device_of(h):
+        mixed = h_type is not None and h_type != x_type
+        dx = h.new_empty(shape, dtype=x_type) if need_x or (need_r and not mixed) else None
+        dres = h.new_empty(shape) if need_r and mixed else None
+        dw = w.new_empty(D) if need_w else None
+        nbytes = lib.odw_rms_norm_bwd_workspace(R, D) if need_w else 0
+        ws = h.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        types = _BF16[x_type] + 2 * _BF16[x_type if h_type is None else h_type] + (4 * _BF16[w.dtype] if w is not None else 0)
+        at = [0 if t is None else t.data_ptr() for t in (g2, d2, h2, w, rstd, dx, dres, dw, ws)]
+        L.check(lib.odw_rms_norm_bwd(at[0], g2.stride(0), at[1], 0 if d2 is None else d2.stride(0), at[2], h2.stride(0), at[3], at[4], R, D,
+                                     at[5], at[6], at[7], types, at[8], nbytes, L.stream()), "rms_norm_bwd")
+    return dx if need_x else None, dw, (dres if mixed else dx) if need_r else None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 def rms_norm(x, weight=None, residual=None, eps=1e-6):
@@ -130,8 +137,8 @@ def rms_norm_fp8(x, weight=None, residual=None, eps=1e-6):
     holds a NaN is all NaN.  No gradients."""
     _check("rms_norm_fp8", x, weight, residual, eps)
     with L.on_device_of(x):
-        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+        scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
         h = _run("rms_norm_fp8", x, weight, residual, eps, q, scale=scale)
     return (q, scale) if h is None else (q, scale, h)
 

@@ -314,6 +314,10 @@ class AdamW(torch.optim.Optimizer):
     def _state(self, p):
         st = self.state[p]
         if not st:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                del self.state[p]
+                raise RuntimeError("AdamW: a parameter's first step is being captured: every replay would start it from zero averages again "
+                                   "(take a step, or load a state, before the capture)")
             if self.state_bits == 8:
                 st["exp_avg"], st["exp_avg_sq"], st["scales"] = state8_zeros(p)
             else:

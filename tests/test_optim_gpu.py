@@ -517,3 +517,37 @@ def test_refusals():
             m[0].add_(1.0)
         finally:
             graph.capture_end()
+
+
+def test_a_first_step_is_not_captured_and_later_ones_are():
+    from od_wscl_amd import optim
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.ones(1000, device="cuda"))
+        ref = torch.nn.Parameter(torch.ones(1000, device="cuda"))
+        p.grad, ref.grad = (torch.linspace(-1, 1, 1000, device="cuda") for _ in range(2))
+        o, r = (optim.AdamW([x], lr=1e-2, state_bits=bits, max_grad_norm=1.0, capturable=True) for x in (p, ref))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph = torch.cuda.CUDAGraph()
+            graph.capture_begin()
+            try:
+                with pytest.raises(RuntimeError, match="first step"):
+                    o.step()
+                p.grad.mul_(1.0)
+            finally:
+                graph.capture_end()
+        torch.cuda.current_stream().wait_stream(side)
+        assert not o.state_dict()["state"]
+        o.step()
+        r.step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o.step()
+        for t in range(4):
+            for x in (p, ref):
+                x.grad.copy_(torch.randn(1000, generator=torch.Generator().manual_seed(t)))
+            graph.replay()
+            r.step()
+            torch.cuda.synchronize()
+            assert torch.equal(p, ref) and float(o.state_dict()["state"][0]["step"]) == t + 2

@@ -273,3 +273,34 @@ def test_module_and_refusals():
                        (lambda: layers.rms_norm_fp8(x.double(), w), TypeError)):
         with pytest.raises(error):
             bad()
+
+
+def test_a_second_derivative_is_refused():
+    from od_wscl_amd import layers
+    x, w = _rand(95, 6, 40).requires_grad_(True), torch.ones(40, device="cuda", requires_grad=True)
+    y = layers.rms_norm(x, w)
+    first, = torch.autograd.grad(y.square().sum(), x, retain_graph=True)
+    gx, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    assert torch.equal(gx, first)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(gx.sum(), x)
+
+
+def test_more_rows_than_a_launch_takes():
+    from od_wscl_amd import layers
+    R = (1 << 23) + 5                                   # (2^21 workgroups of four rows)
+    x, r, w = _rand(96, R, 3), _rand(97, R, 3), 1 + _rand(98, 3)
+    y, h = layers.rms_norm(x, w, residual=r, eps=EPS)
+    q, s, h2 = layers.rms_norm_fp8(x, w, residual=r, eps=EPS)
+    rh, _, ry = _reference(x, w, r)
+    assert torch.equal(h.double(), rh) and torch.equal(h2, h)
+    _near(y, ry, _sum_ulps(3) + HALF[F32])
+    _near(s, ry.abs().amax(1) / 448, _sum_ulps(3) + 4 * U32)
+    assert (q.float().abs().amax(1) == 448).all()
+    xs, ws = x.requires_grad_(True), w.requires_grad_(True)
+    dx, dw = torch.autograd.grad(layers.rms_norm(xs, ws, residual=r, eps=EPS)[0], (xs, ws), r)
+    tail = x.detach()[-7:].requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(layers.rms_norm(tail, w, residual=r[-7:], eps=EPS)[0], tail, r[-7:])[0], dx[-7:])
+    rs = 1 / torch.sqrt((rh * rh).mean(-1, keepdim=True) + EPS)
+    # (2048 groups of 4097 rows each and 2048 partial sums: all in fp32)
+    assert ((dw.double() - (r.double() * rh * rs).sum(0)).abs() <= (4097 + 2048 + 16) * U32 * (r.double() * rh * rs).abs().sum(0)).all()
