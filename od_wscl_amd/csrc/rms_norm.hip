@@ -152,13 +152,45 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x, float* part) {
     return x;
 }
 
-template <class TX, class TH, int TPR, int VPT, int V, bool PAST>
+// The 8-bit codes are the correctly rounded ones, q = rne(y / (max |y| / 448)), where a quotient rounded to fp32 on the way would go the other
+// way round a few times in a million.  The row's factor cancels in it: with t = h w, q = rne(448 t / max |t|).  The fp32 quotient z stands for
+// an interval; a thread rounds both its ends, and only rows with a code that is open then go the long way for those codes: t = p + e
+// exactly (p the rounded product, e its error by one fma), 448 / max |t| = c + cl in two fp32 numbers, and the product's first 24 bits in f,
+// the rest in the sign of lo: f with its last bit standing for "and something more" (rounding to odd) rounds to 8 bits as the exact product.
+// (Every element the long way: 2000 x 25088 fp32 76 us.)
+__device__ __forceinline__ float times_to_odd(float h, float w, float c, float cl) {
+    const float p = h * w, e = fmaf(h, w, -p), z = p * c;
+    const float r = fmaf(e, c, fmaf(p, cl, fmaf(p, c, -z)));
+    const float f = z + r, lo = r - (f - z);
+    uint32_t u = __float_as_uint(f);
+    // (c + cl and r are good to 2^-47: nearer to a tie than 2^-44 is a tie)
+    if (fabsf(lo) > fabsf(f) * 0x1p-44f) u = (((__float_as_uint(lo) ^ u) >> 31) ? u - 1u : u) | 1u;
+    return __uint_as_float(u);
+}
+__device__ __forceinline__ int codes4(float z0, float z1, float z2, float z3) {
+    return __builtin_amdgcn_cvt_pk_fp8_f32(z2, z3, __builtin_amdgcn_cvt_pk_fp8_f32(z0, z1, 0, false), true);
+}
+__device__ __forceinline__ void store_codes(uint8_t* q, int left, int u) {
+    typedef int word __attribute__((aligned(1)));
+    if (left >= 4) {
+        *reinterpret_cast<word*>(q) = u;
+    } else {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            if (b < left) q[b] = (uint8_t)(u >> (8 * b));
+    }
+}
+
+// OUT8: `scale` is given and y are the codes.  (The branch on `scale` is uniform and decided by OUT8; left to run time it keeps what belongs to a
+// vector together -- without it the scheduler loads the whole row's weight ahead: 2000 x 25088 bf16 92 us for 78, its registers spilt.)
+template <class TX, class TH, int TPR, int VPT, int V, bool PAST, bool OUT8>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1) void rms_norm_row_kernel(const TX* __restrict__ x, int64_t ldx, const TH* __restrict__ res,
                                                                              int64_t ldr, const void* __restrict__ w, int64_t R, int D, float eps,
-                                                                             void* __restrict__ y, TH* __restrict__ h, float* __restrict__ rstd,
+                                                                             void* __restrict__ y, TH* h, float* __restrict__ rstd,
                                                                              float* __restrict__ scale, int types) {
     constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
     __shared__ float part[2][TPR > 64 ? TPR / 64 : 1];
+    __shared__ int any[TPR > 64 ? TPR / 64 : 1];
     static_assert(TPR == 64 || kRows == 1, "rows that share a workgroup have a wave each");
     const int t = kRows == 1 ? threadIdx.x : threadIdx.x % TPR;
     // (a wave's row is uniform, and the compiler has to know it: scalar row addresses)
@@ -196,49 +228,90 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1) void rms_
     s = row_sum<TPR>(s, part[0]);
     const float rs = 1.0f / sqrtf(s / (float)D + eps);
     if (rstd && t == 0) rstd[r] = rs;
-    uint32_t top = 0;
+    uint32_t best = 0;                           // (8 bits) the largest word of the products' magnitudes: a NaN's is above all numbers'
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         const int i = (k * TPR + t) * V;
         if (i < D) {
             float g[V];
             load_w<V>(w, types & kWBf16, i, D - i, g);
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[k][j] = v[k][j] * rs * g[j];
             if (!scale) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[k][j] = v[k][j] * rs * g[j];
                 store<TX, V, PAST>((TX*)y + r * D + i, D - i, v[k]);
             } else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
+                    v[k][j] *= g[j];
                     const uint32_t u = __float_as_uint(v[k][j]) & 0x7FFFFFFFu;
-                    top = top > u ? top : u;
+                    best = best > u ? best : u;
                 }
             }
         }
     }
-    if (!scale) return;
-    // the largest word of the magnitudes: a NaN's is above all numbers', so it makes the scale and the whole row NaN
-    const float sc0 = __uint_as_float(row_max<TPR>(top, part[1])) / 448.0f;
-    const float sc = sc0 < 1.17549435e-38f ? 1.17549435e-38f : sc0, inv = 1.0f / sc;
+    if (!OUT8 || !scale) return;
+    const float pm = __uint_as_float(row_max<TPR>(best, part[1]));
+    const float sc0 = pm * rs / 448.0f;
+    const float sc = sc0 < 1.17549435e-38f ? 1.17549435e-38f : sc0;
     if (t == 0) scale[r] = sc;
+    // far off, infinite, NaN (it makes the scale and the whole row NaN) or held up by the smallest scale: by fp32, as it comes
+    const bool plain = !(pm > 1e-30f && pm < 1e30f) || sc != sc0;
+    const float c = plain ? 1.0f / sc : 448.0f / pm;
+    if (plain)
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-        const int i = (k * TPR + t) * V;
-        if (i >= D) continue;
-        uint8_t* q = (uint8_t*)y + r * D + i;
-        typedef int word __attribute__((aligned(1)));
+        for (int k = 0; k < VPT; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[k][j] *= rs;
+    // (z is off by at most 4 * 2^-24 of itself: the product, the largest product, the quotient, their product)
+    const float under = plain ? c : c * (1.0f - 0x1p-21f), over = plain ? c : c * (1.0f + 0x1p-21f);
+    uint32_t open = 0;                           // fours whose codes are open
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
 #pragma unroll
         for (int j = 0; j < V; j += 4) {
-            int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][j] * inv, v[k][j + 1] * inv, 0, false);
-            u = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][j + 2] * inv, v[k][j + 3] * inv, u, true);
-            if (D - i >= j + 4) {
-                *reinterpret_cast<word*>(q + j) = u;
-            } else {
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-                    if (i + j + b < D) q[j + b] = (uint8_t)(u >> (8 * b));
-            }
+            const int i = (k * TPR + t) * V + j;
+            if (i >= D) continue;
+            const int u = codes4(v[k][j] * under, v[k][j + 1] * under, v[k][j + 2] * under, v[k][j + 3] * under);
+            if (u != codes4(v[k][j] * over, v[k][j + 1] * over, v[k][j + 2] * over, v[k][j + 3] * over)) open |= 1u << (k * (V / 4) + j / 4);
+            store_codes((uint8_t*)y + r * D + i, D - i, u);
         }
+    bool some = __any(open != 0);
+    if (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) any[threadIdx.x >> 6] = some;
+        __syncthreads();
+        some = false;
+#pragma unroll
+        for (int k = 0; k < TPR / 64; ++k) some |= any[k] != 0;
+    }
+    if (!some) return;
+    // (the values again, from where they came: their registers hold the products)
+    auto value = [&](int i) { return res ? up(h[r * D + i]) : up(x[r * ldx + i]); };
+    auto gain = [&](int i) { return w ? ld(w, types & kWBf16, i) : 1.0f; };
+    // e of the largest product (of equal ones the largest e; of equal ones in one thread the last one's), as a word that grows with it
+    uint32_t key = 0;
+    if (best == __float_as_uint(pm)) {
+        int at = 0;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if ((__float_as_uint(v[k][j]) & 0x7FFFFFFFu) == best) at = (k * TPR + t) * V + j;
+        const float hv = value(at), gv = gain(at), p = hv * gv;
+        const uint32_t e = __float_as_uint(p < 0.0f ? -fmaf(hv, gv, -p) : fmaf(hv, gv, -p));
+        key = (e >> 31) ? ~e : e | 0x80000000u;
+    }
+    key = row_max<TPR>(key, part[0]);
+    const double tmax = (double)pm + (double)__uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
+    const double cd = 448.0 / tmax;
+    const float ch = (float)cd, cl = (float)(cd - (double)ch);
+#pragma clang loop unroll(disable)
+    while (open) {
+        const int n = __ffs(open) - 1, i = ((n / (V / 4)) * TPR + t) * V + (n % (V / 4)) * 4;
+        open &= open - 1;
+        float z[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) z[b] = i + b < D ? times_to_odd(value(i + b), gain(i + b), ch, cl) : 0.0f;
+        store_codes((uint8_t*)y + r * D + i, D - i, codes4(z[0], z[1], z[2], z[3]));
     }
 }
 
@@ -488,7 +561,10 @@ void forward(const void* x, int64_t ldx, const void* res, int64_t ldr, const voi
     auto launch = [&](auto s) {
         typedef decltype(s) S;
         constexpr int kRows = S::tpr > 256 ? 1 : 256 / S::tpr;
-        const auto kernel = past ? rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v, true> : rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v, false>;
+        const auto kernel = scale ? (past ? rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v, true, true>
+                                          : rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v, false, true>)
+                                  : (past ? rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v, true, false>
+                                          : rms_norm_row_kernel<TX, TH, S::tpr, S::vpt, S::v, false, false>);
         // (a launch has fewer than 2^32 threads: rows beyond go to further ones)
         constexpr int64_t kMost = (int64_t)1 << 21;
         for (int64_t r = 0; r < R; r += kMost * kRows) {

@@ -133,8 +133,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
 @torch.no_grad()
 def rms_norm_fp8(x, weight=None, residual=None, eps=1e-6):
     """rms_norm with its output in 8 bits: (q, scale), or (q, scale, h) with a residual.  q float8_e4m3fn of x's shape, scale fp32 (...,):
-    y ~ q.float() * scale[..., None], scale = max |y| / 448 of the row (2^-126 for a row of zeros); rounded to nearest even.  A row that
-    holds a NaN is all NaN.  No gradients."""
+    y ~ q.float() * scale[..., None], scale = max |y| / 448 of the row (2^-126 for a row of zeros).  q is the quotient correctly
+    rounded (ties to even); in rows over 32768 elements it is rounded to fp32 first.  A row that holds a NaN is all NaN.  No gradients."""
     _check("rms_norm_fp8", x, weight, residual, eps)
     with L.on_device_of(x):
         q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)

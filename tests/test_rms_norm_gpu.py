@@ -304,3 +304,34 @@ def test_more_rows_than_a_launch_takes():
     rs = 1 / torch.sqrt((rh * rh).mean(-1, keepdim=True) + EPS)
     # (2048 groups of 4097 rows each and 2048 partial sums: all in fp32)
     assert ((dw.double() - (r.double() * rh * rs).sum(0)).abs() <= (4097 + 2048 + 16) * U32 * (r.double() * rh * rs).abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("R,D", [s for s in SHAPES if s[1] <= 32768] + [(2000, 4100), (300, 25088)])
+@pytest.mark.parametrize("xt,wt", [(F32, F32), (BF16, F32), (F32, None), (BF16, BF16)])
+def test_8_bit_codes_are_the_correctly_rounded_ones(R, D, xt, wt):
+    """rne(448 t / max |t|), t = h w: the products and their quotient in fp64 (off by 2^-52: an element would have to lie that near to the
+    middle of two codes, and one that lies on it goes to the even code on both sides)."""
+    from od_wscl_amd import layers
+    x, res, w = _case(R, D, xt, xt, wt, seed=120)
+    q, _, h = layers.rms_norm_fp8(x, w, residual=res, eps=EPS)
+    t = h.double().cpu().numpy() * (w.double().cpu().numpy() if w is not None else 1.0)
+    z = 448 * t / np.abs(t).max(1, keepdims=True)
+    e = np.maximum(np.frexp(z)[1] - 1, -6)
+    want = np.ldexp(np.rint(np.ldexp(z, 3 - e)), e - 3)          # (torch.ldexp and ** go through pow on the GPU: off by an ulp)
+    assert np.array_equal(q.float().cpu().numpy(), want)
+
+
+def test_8_bit_rows_of_any_size():
+    """Rows scaled by powers of two from 2^-140 to 2^50 hold the same codes wherever fp32 can form them: the scale takes the factor (eps is in
+    its way below 2^-10, so the row's factor there is 1 / sqrt(eps), and 2^-126 is the smallest scale)."""
+    from od_wscl_amd import layers
+    base = _rand(130, 1, 1000)
+    q0, s0 = layers.rms_norm_fp8(base, eps=EPS)
+    for k in (-140, -120, -100, -60, -20, -8, 8, 30, 50):
+        x = base * 2.0 ** k if k > -100 else base * 2.0 ** -100 * 2.0 ** (k + 100)
+        q, s = layers.rms_norm_fp8(x, eps=EPS)
+        y = _reference(x, None, None)[2]
+        assert s.item() >= 2.0 ** -126 and torch.isfinite(q.float()).all()
+        assert ((q.double() * s.double() - y).abs() <= y.abs() * (2.0 ** -4 + 2.0 ** -20) + s.double() * 2.0 ** -10 + 2.0 ** -149).all(), k
+        if -100 <= k:
+            assert torch.equal(q.float(), q0.float()), k
