@@ -4,6 +4,10 @@
 // A launch takes up to kMaxTensors tensors: their pointers and sizes travel in the kernel's arguments (no table in device
 // memory to upload, nothing to keep alive for a captured launch).  The tensors are cut into chunks; a
 // workgroup finds the tensor of its chunk by bisection over the chunks' prefix -- the index is uniform, so this is scalar work.
+//
+// Both are bound by the bytes: an element's update is ~20 operations on 28 bytes with fp32 states (30 with a bf16 copy of p), ~70 on 16
+// (18) with 8-bit ones.  153 M parameters in 42 tensors with copies: 796 us (5.8 TB/s) and 463 us (5.9 TB/s); their gradients' norm
+// 88 us (7.0 TB/s), their scaling 220 us (5.5 TB/s).  A launch of a million elements takes 10-12 us.
 #include "odw_common.h"
 #include "odw_rng.h"
 #include <math.h>
