@@ -1,7 +1,7 @@
 // adamw.hip -- the AdamW update of many tensors in one launch (states in fp32, or in 8-bit floats with block scales), and the
 // global gradient norm it is clipped by.
 //
-// A launch takes up to kMaxTensors tensors: their pointers and sizes travel in the kernel's arguments (no table in device
+// A launch takes up to kMaxTensors tensors (the norm kNormTensors): their pointers and sizes travel in the kernel's arguments (no table in device
 // memory to upload, nothing to keep alive for a captured launch).  The tensors are cut into chunks; a
 // workgroup finds the tensor of its chunk by bisection over the chunks' prefix -- the index is uniform, so this is scalar work.
 //
@@ -14,7 +14,7 @@
 
 namespace {
 
-constexpr int kMaxTensors = 44;          // (88 B each: the arguments stay under 4 KB)
+constexpr int kMaxTensors = 48, kNormTensors = 160;      // (the arguments stay under 4 KB)
 constexpr int kBlock = 256;              // elements that share a scale: one wave, four elements a lane
 // A workgroup's four waves have a whole chunk's loads in flight: 4 blocks a wave of fp32 states, 2 of 8-bit ones (more registers a
 // block).  153 M parameters with bf16 copies, us: fp32 states 825 (2 blocks), 796 (4), 819 (8); 8-bit states 493 (1), 468 (2), 475 (4); chunks
@@ -52,12 +52,13 @@ struct Args {
 };
 
 struct NormArgs {
-    const void* g[kMaxTensors];
-    int64_t n[kMaxTensors];
-    int chunk0[kMaxTensors];
-    uint8_t flags[kMaxTensors];
+    const void* g[kNormTensors];
+    int64_t n[kNormTensors];
+    int chunk0[kNormTensors];
+    uint8_t flags[kNormTensors];
     int count, chunks;
 };
+static_assert(sizeof(Args) <= 4096 && sizeof(NormArgs) <= 4096 - 64, "kernel arguments");
 
 __device__ __forceinline__ float bf2f(unsigned short h) { return __uint_as_float((uint32_t)h << 16); }
 __device__ __forceinline__ unsigned short f2bf(float f) {      // round to nearest even; NaN stays NaN
@@ -436,7 +437,7 @@ constexpr int64_t kMaxElements = (int64_t)1 << 40;           // of one tensor: i
 // Fills `a` with tensors from `i` on (empty ones left out) until it is full; returns the first one not taken.
 int fill_norm_args(NormArgs& a, int i, int n_tensors, const void* const* g, const int64_t* n, const int* types) {
     a.count = a.chunks = 0;
-    for (; i < n_tensors && a.count < kMaxTensors; ++i) {
+    for (; i < n_tensors && a.count < kNormTensors; ++i) {
         if (n[i] == 0) continue;
         if (a.count && a.chunks + chunks_of(n[i], kNormChunk) > INT32_MAX) break;
         a.g[a.count] = g[i];

@@ -66,6 +66,16 @@ def _types(tensors):
     return [_TYPES[kinds.pop()]] * len(tensors) if len(kinds) == 1 else [_TYPES[t.dtype] for t in tensors]
 
 
+def _changed(tensors):
+    """Tell autograd that they were written (tensors made in inference mode have no version to count)."""
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:
+        for t in tensors:
+            if not t.is_inference():
+                torch.autograd.graph.increment_version([t])
+
+
 class _Lists(object):
     """Host arrays for a call of the library, alive until it returns (it reads them before that)."""
 
@@ -148,7 +158,7 @@ def clip_grad_norm_(grads, max_norm):
     max_norm; returns the norm before that (torch.nn.utils.clip_grad_norm_, without a host read)."""
     grads = _grads_of("clip_grad_norm_", grads)
     out = _norm("clip_grad_norm_", grads, float(max_norm), written=True)
-    torch.autograd.graph.increment_version(grads)
+    _changed(grads)
     return out[0]
 
 
@@ -192,7 +202,7 @@ def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_
             _device_scalar(what, "step", step, device, torch.int64)
             bias = torch.empty(4, dtype=torch.float32, device=params[0].device)
             L.check(lib.odw_adamw_advance(L.ptr(step), betas[0], betas[1], L.ptr(bias), L.stream()), "adamw_advance")
-            torch.autograd.graph.increment_version([step])
+            _changed([step])
             number = 0
         else:
             number = int(step)
@@ -209,13 +219,13 @@ def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_
         else:
             L.check(lib.odw_adamw(*head, *tail, max_workgroups, L.stream()), what)
     for _, tensors, _ in written:
-        torch.autograd.graph.increment_version(tensors)
+        _changed(tensors)
 
 
 @torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, grad_scale=None,
                copies=None, grad_mult=1.0, max_workgroups=0):
-    """One AdamW step over lists of tensors, in place, one launch for up to 44 of them:
+    """One AdamW step over lists of tensors, in place, one launch for up to 48 of them:
 
         g' = g * grad_mult * grad_scale
         m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2

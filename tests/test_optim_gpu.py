@@ -551,3 +551,25 @@ def test_a_first_step_is_not_captured_and_later_ones_are():
             r.step()
             torch.cuda.synchronize()
             assert torch.equal(p, ref) and float(o.state_dict()["state"][0]["step"]) == t + 2
+
+
+def test_norm_of_more_tensors_than_a_launch_takes():
+    from od_wscl_amd import optim
+    sizes = [int(x) for x in np.random.RandomState(1).randint(0, 3000, 401)] + [70000]
+    g = _lists(sizes, 12, gt=BF16, packed=True)[1]
+    want = math.sqrt(sum(float((x.double() ** 2).sum()) for x in g))
+    ref = [x.clone() for x in g]
+    norm, coef = optim.grad_norm(g, max_norm=1.0)
+    assert abs(norm.item() / want - 1) <= 2 * U
+    assert torch.equal(optim.clip_grad_norm_(g, 1.0), norm)
+    assert all(torch.equal(a, (b.float() * coef).to(BF16)) for a, b in zip(g, ref))
+
+
+def test_tensors_made_in_inference_mode():
+    from od_wscl_amd import layers, optim
+    with torch.inference_mode():
+        p, g, m, v = (torch.ones(300, device="cuda") for _ in range(4))
+        optim.adamw_step([p], [g], [m], [v], 1, lr=0.5)
+        optim.clip_grad_norm_([g], 1.0)
+        y, h = layers.rms_norm(p.view(3, 100), g[:100], residual=v.view(3, 100))
+    assert (p < 1).all() and abs(g.norm().item() - 1) < 1e-5 and torch.isfinite(y).all()
