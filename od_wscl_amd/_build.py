@@ -1,4 +1,4 @@
-"""Builds libodwscl.so (every HIP kernel + the C-ABI) for gfx950, in-tree.
+"""Builds libodwscl.so (every HIP kernel + the C-ABI) for gfx950 and _bind.so (torch-side glue in front of it), in-tree.
 
 hipcc cross-compiles without a GPU, so this also runs in the CPU-only build
 container; the resulting .so is git-ignored but ships with gpurun snapshots.
@@ -10,6 +10,7 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libodwscl.so")
+BIND, BIND_SRC = os.path.join(HERE, "_bind.so"), os.path.join(CSRC, "bind.cpp")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 # -ffp-contract=off: ROI bin / sample coordinates must round exactly like the
@@ -30,17 +31,29 @@ def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.hip")))
 
 
+def _bind_command():
+    """Host code only: the C++ compiler, torch's headers and the HIP headers that those include."""
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), "/opt/rocm/include"]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch.compiled_with_cxx11_abi())] + [f for i in inc for f in ("-isystem", i)] +
+            ["-I" + sysconfig.get_paths()["include"], BIND_SRC, "-o", BIND, "-L" + HERE, "-l:" + os.path.basename(LIB), "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu",
+             "-ltorch", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN"])
+
+
 def _stale():
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(BIND):
         return True
-    t = os.path.getmtime(LIB)
-    deps = sources() + glob.glob(os.path.join(CSRC, "*.h")) + \
+    t = min(os.path.getmtime(LIB), os.path.getmtime(BIND))
+    deps = sources() + [BIND_SRC] + glob.glob(os.path.join(CSRC, "*.h")) + \
         glob.glob(os.path.join(HERE, "..", "include", "*.h"))
     return any(os.path.getmtime(p) > t for p in deps)
 
 
 def build(force=False, verbose=False):
-    """Compile csrc/*.hip -> libodwscl.so (objects cached next to the sources)."""
+    """Compile csrc/*.hip -> libodwscl.so (objects cached next to the sources), csrc/bind.cpp -> _bind.so."""
     if not force and not _stale():
         return LIB
     objs = []
@@ -64,6 +77,14 @@ def build(force=False, verbose=False):
             print(out.decode())
     cmd = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", LIB] + objs
     subprocess.check_call(cmd)
+    newest = max(os.path.getmtime(p) for p in [BIND_SRC] + glob.glob(os.path.join(HERE, "..", "include", "*.h")))
+    if force or not os.path.exists(BIND) or os.path.getmtime(BIND) <= newest:
+        cmd = _bind_command()
+        if verbose:
+            print(" ".join(cmd))
+        subprocess.check_call(cmd)
+    else:
+        os.utime(BIND)
     return LIB
 
 

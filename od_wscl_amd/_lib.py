@@ -6,7 +6,6 @@ written gfx950 kernels.  There is NO fallback: if the shared object is missing
 or a tensor is not on the GPU the call raises (the reference raises
 "Not implemented on the CPU" the same way, csrc/ROIPool.h:23).
 """
-import contextlib
 import ctypes
 import os
 
@@ -14,6 +13,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libodwscl.so")
+BIND_PATH = os.path.join(_HERE, "_bind.so")
 _lib = None
 
 c_d = ctypes.c_double
@@ -236,16 +236,20 @@ def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-_no_guard = contextlib.nullcontext()
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_bind = None
 
 
-def on_device_of(t):
-    """Context in which the current device is t's (launches go to the current device's current stream); nothing to do in the usual
-    case that it is already."""
-    index = t.get_device()
-    # (t is on a GPU, so the runtime is up: its own query, a tenth of torch.cuda.current_device())
-    return _no_guard if index == _current_device() else torch.cuda.device(index)
+def bind():
+    """The torch-side glue of the optimiser and the row norm (csrc/bind.cpp -> _bind.so, which calls libodwscl.so); raises if it was never
+    built."""
+    global _bind
+    if _bind is None:
+        lib()
+        if not os.path.exists(BIND_PATH):
+            raise RuntimeError("_bind.so is missing (%s): build it with `python -m od_wscl_amd._build`" % BIND_PATH)
+        from . import _bind as module
+        _bind = module
+    return _bind
 
 
 def ptr(t):

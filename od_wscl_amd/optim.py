@@ -12,7 +12,6 @@ the second in float8_e5m2, a power-of-two scale each for every 256 consecutive e
 counter-based stream of utils/rng.py -- a step is a function of its inputs and its key, whatever the launch geometry.
 
 Every tensor is on one GPU; the work goes to the current stream of that device; nothing is read back to the host."""
-import array
 import math
 
 import torch
@@ -21,208 +20,23 @@ from . import _lib as L
 from .utils import rng
 
 BLOCK = 256          # elements that share a scale of the 8-bit states
-# a gradient whose square is nothing in fp32 (below 1e-21) then moves p by at most lr * 1e-6, not by lr * g / eps of any size
-MIN_EPS = 1e-15
-_TYPES = {torch.float32: 0, torch.bfloat16: 1}
-_FLOATS, _F32, _BF16 = {torch.float32, torch.bfloat16}, {torch.float32}, {torch.bfloat16}
-_M8, _V8, _BYTES = {torch.float8_e4m3fn}, {torch.float8_e5m2}, {torch.uint8}
+MIN_EPS = 1e-15      # (a smaller eps is refused: csrc/bind.cpp says why)
 
 
-_numel, _device, _address, _dense = torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
-_dtype = torch.Tensor.dtype.__get__
-
-
-def _check_list(what, name, tensors, device, sizes, dtypes):
-    """`tensors` beside the first list: as many, on the same GPU, contiguous, of one of `dtypes` and of `sizes`; returns their addresses.
-    (Checked list by list: a call over a hundred tensors costs the host a third of one that looks at each by itself.)"""
-    if (list(map(_numel, tensors)) == sizes and set(map(_device, tensors)) == {device} and set(map(_dtype, tensors)) <= dtypes
-            and all(map(_dense, tensors))):
-        return list(map(_address, tensors))
-    if len(tensors) != len(sizes):
-        raise ValueError("%s: %d %s for %d tensors" % (what, len(tensors), name, len(sizes)))
-    L.need_gpu(*tensors)
-    for i, (t, n) in enumerate(zip(tensors, sizes)):
-        if t.get_device() != device:
-            raise ValueError("%s: %s[%d] is on %s, tensor 0 on cuda:%d" % (what, name, i, t.device, device))
-        if t.dtype not in dtypes:
-            raise TypeError("%s: %s[%d] is %s (%s)" % (what, name, i, t.dtype, " | ".join(str(d) for d in dtypes)))
-        if t.numel() != n:
-            raise ValueError("%s: %s[%d] has %d elements, %d wanted" % (what, name, i, t.numel(), n))
-        if not t.is_contiguous():
-            raise ValueError("%s: %s[%d] is not contiguous" % (what, name, i))
-
-
-def _distinct(what, name, at):
-    """A tensor that is written must not be in the list twice (two workgroups would update it at once); empty ones have address 0."""
-    seen = set(at)
-    if len(seen) != len(at):
-        seen.discard(0)
-        if len(seen) != len(at) - at.count(0):
-            raise ValueError("%s: the same tensor is in `%s` twice" % (what, name))
-
-
-def _types(tensors):
-    kinds = set(map(_dtype, tensors))
-    return [_TYPES[kinds.pop()]] * len(tensors) if len(kinds) == 1 else [_TYPES[t.dtype] for t in tensors]
-
-
-def _changed(tensors):
-    """Tell autograd that they were written (tensors made in inference mode have no version to count)."""
-    try:
-        torch.autograd.graph.increment_version(tensors)
-    except RuntimeError:
-        for t in tensors:
-            if not t.is_inference():
-                torch.autograd.graph.increment_version([t])
-
-
-class _Lists(object):
-    """Host arrays for a call of the library, alive until it returns (it reads them before that)."""
-
-    def __init__(self):
-        self.kept = []
-
-    def __call__(self, code, values):
-        a = array.array(code, values)
-        self.kept.append(a)
-        return a.buffer_info()[0] or None
-
-
-def _scalar_list(what, name, value, n):
-    if isinstance(value, (int, float)):
-        value = (value,) * n
-    if len(value) != n:
-        raise ValueError("%s: %d values of %s for %d tensors" % (what, len(value), name, n))
-    for x in set(value):
-        if not (x >= 0.0 and math.isfinite(x)):
-            raise ValueError("%s: %s = %r" % (what, name, x))
-    return value
-
-
-def _device_scalar(what, name, t, device, dtype):
-    if t.numel() != 1 or t.dtype != dtype or t.get_device() != device:
-        raise ValueError("%s: %s has to be one %s on cuda:%d (got %s of %d elements on %s)" % (what, name, dtype, device, t.dtype, t.numel(), t.device))
-
-
-def _grads_of(what, items):
-    """Gradients out of a list of tensors and / or parameters: a leaf that requires grad stands for its .grad."""
-    grads = []
-    for t in items:
-        if t.requires_grad and t.is_leaf:
-            if t.grad is not None:
-                grads.append(t.grad)
-        else:
-            grads.append(t)
-    for i, g in enumerate(grads):
-        if g.is_sparse:
-            raise TypeError("%s: gradient %d is sparse" % (what, i))
-    return grads
-
-
-def _norm(what, grads, max_norm, written=False):
-    if not grads:
-        raise ValueError("%s: no gradients" % what)
-    L.need_gpu(grads[0])
-    sizes = list(map(_numel, grads))
-    at = _check_list(what, "grads", grads, grads[0].get_device(), sizes, _FLOATS)
-    if written:
-        _distinct(what, "grads", at)
-    if not max_norm > 0.0:
-        raise ValueError("%s: max_norm = %r" % (what, max_norm))
-    lib, lists, count = L.lib(), _Lists(), len(grads)
-    head = (count, lists("Q", at), lists("q", sizes), lists("i", [2 * t for t in _types(grads)]))
-    with L.on_device_of(grads[0]):
-        nbytes = lib.odw_grad_norm_workspace(count, head[2])
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device) if nbytes else None
-        out = torch.empty(2, dtype=torch.float32, device=grads[0].device)
-        L.check(lib.odw_grad_norm(*head, max_norm, L.ptr(out), L.ptr(ws), nbytes, L.stream()), "grad_norm")
-        if written:
-            L.check(lib.odw_scale_tensors(*head, out.data_ptr() + 4, L.stream()), "scale_tensors")
-    return out
-
-
-@torch.no_grad()
 def grad_norm(grads, max_norm=None):
     """The 2-norm over all of `grads` (tensors, or parameters that stand for their .grad) as a 0-dim fp32 tensor; summed in fp64 in
     one order, so the same from run to run.  With max_norm: (norm, coef), coef = min(1, max_norm / (norm + 1e-6)) -- the factor
     that clips them, for `grad_scale` of adamw_step (clipping without a pass over the gradients).  Neither is read by the host.
     A non-finite gradient makes the norm inf or NaN, and coef 0 or NaN."""
-    grads = [g if g.is_contiguous() else g.contiguous() for g in _grads_of("grad_norm", grads)]
-    out = _norm("grad_norm", grads, math.inf if max_norm is None else float(max_norm))
-    return out[0] if max_norm is None else (out[0], out[1])
+    return L.bind().grad_norm(list(grads), max_norm)
 
 
-@torch.no_grad()
 def clip_grad_norm_(grads, max_norm):
     """Scale all of `grads` (tensors, or parameters that stand for their .grad) in place so that their common 2-norm is at most
     max_norm; returns the norm before that (torch.nn.utils.clip_grad_norm_, without a host read)."""
-    grads = _grads_of("clip_grad_norm_", grads)
-    out = _norm("clip_grad_norm_", grads, float(max_norm), written=True)
-    _changed(grads)
-    return out[0]
+    return L.bind().clip_grad_norm(list(grads), max_norm)
 
 
-def _step(bits8, params, grads, m, v, scales, step, key, lr, betas, eps, weight_decay, grad_scale, copies, grad_mult, max_workgroups):
-    what = "adamw8_step" if bits8 else "adamw_step"
-    if not params:
-        return
-    L.need_gpu(params[0])
-    count, device, sizes = len(params), params[0].get_device(), list(map(_numel, params))
-    ap, ag = _check_list(what, "params", params, device, sizes, _FLOATS), _check_list(what, "grads", grads, device, sizes, _FLOATS)
-    am = _check_list(what, "exp_avgs", m, device, sizes, _M8 if bits8 else _F32)
-    av = _check_list(what, "exp_avg_sqs", v, device, sizes, _V8 if bits8 else _F32)
-    written = [("params", params, ap), ("exp_avgs", m, am), ("exp_avg_sqs", v, av)]
-    if bits8:
-        ae = _check_list(what, "scales", scales, device, [2 * (-(-n // BLOCK)) for n in sizes], _BYTES)
-        written.append(("scales", scales, ae))
-    ac = None
-    if copies is not None:
-        if len(copies) != count:
-            raise ValueError("%s: %d copies for %d tensors" % (what, len(copies), count))
-        have = [c for c in copies if c is not None]
-        if have:
-            at = _check_list(what, "copies", have, device, [n for n, c in zip(sizes, copies) if c is not None], _BF16)
-            written.append(("copies", have, at))
-            at = iter(at)
-            ac = [0 if c is None else next(at) for c in copies]
-    for name, _, at in written:
-        _distinct(what, name, at)
-    if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
-        raise ValueError("%s: betas = %r" % (what, betas))
-    if not (eps >= MIN_EPS and math.isfinite(eps)):
-        raise ValueError("%s: eps = %r" % (what, eps))
-    if not math.isfinite(grad_mult):
-        raise ValueError("%s: grad_mult = %r" % (what, grad_mult))
-    lr, weight_decay = _scalar_list(what, "lr", lr, count), _scalar_list(what, "weight_decay", weight_decay, count)
-    if grad_scale is not None:
-        _device_scalar(what, "grad_scale", grad_scale, device, torch.float32)
-    lib, bias, lists = L.lib(), None, _Lists()
-    with L.on_device_of(params[0]):
-        if torch.is_tensor(step):
-            _device_scalar(what, "step", step, device, torch.int64)
-            bias = torch.empty(4, dtype=torch.float32, device=params[0].device)
-            L.check(lib.odw_adamw_advance(L.ptr(step), betas[0], betas[1], L.ptr(bias), L.stream()), "adamw_advance")
-            _changed([step])
-            number = 0
-        else:
-            number = int(step)
-            if number < 1 or number != step:
-                raise ValueError("%s: step = %r (the first one is 1)" % (what, step))
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("%s: a captured step would replay step %d for ever: pass `step` as an int64 tensor on the GPU" % (what, number))
-        head = (count, lists("Q", ap), lists("Q", ag), lists("Q", am), lists("Q", av))
-        tail = (lists("Q", ac) if ac is not None else None, lists("q", sizes),
-                lists("i", [tp + 2 * tg for tp, tg in zip(_types(params), _types(grads))]), lists("f", lr), lists("f", weight_decay),
-                betas[0], betas[1], eps, number, L.ptr(bias), L.ptr(grad_scale), grad_mult)
-        if bits8:
-            L.check(lib.odw_adamw8(*head, lists("Q", ae), *tail, key[0], key[1], max_workgroups, L.stream()), what)
-        else:
-            L.check(lib.odw_adamw(*head, *tail, max_workgroups, L.stream()), what)
-    for _, tensors, _ in written:
-        _changed(tensors)
-
-
-@torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, grad_scale=None,
                copies=None, grad_mult=1.0, max_workgroups=0):
     """One AdamW step over lists of tensors, in place, one launch for up to 48 of them:
@@ -236,11 +50,10 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     tensor on the GPU that holds the steps taken and is advanced here, the form a HIP graph can capture.  grad_scale: one fp32 on the
     GPU (the clip coefficient of grad_norm).  copies: list of bf16 tensors (or None) that get the new params, as the matrix cores read
     them.  max_workgroups: 0, or the width of a pass that runs beside other work."""
-    _step(False, params, grads, exp_avgs, exp_avg_sqs, None, step, None, lr, betas, eps, weight_decay, grad_scale, copies, grad_mult,
-          max_workgroups)
+    L.bind().adamw(False, params, grads, exp_avgs, exp_avg_sqs, None, step, (), lr, betas, eps, weight_decay, grad_scale, copies, grad_mult,
+                   max_workgroups)
 
 
-@torch.no_grad()
 def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, scales, step, key, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                 grad_scale=None, copies=None, grad_mult=1.0, max_workgroups=0):
     """adamw_step with 8-bit states: exp_avgs float8_e4m3fn, exp_avg_sqs float8_e5m2, scales uint8 (ceil(n / 256), 2): exponent + 127 of
@@ -248,10 +61,8 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, scales, step, key, lr=1e-3
     state8_write); a second average that is not zero is held as 2^-16 of its scale at least.  The update uses the averages before they are rounded.  key: two 32-bit integers, other ones every step
     (utils.rng.stream_key(seed, step)); the random bits of an element depend on the key and on its position in the concatenation of
     `params`.  With `step` on the GPU the step's number is added to key[1].  An average that is not finite is held as NaN."""
-    if len(key) != 2 or not all(0 <= int(k) < (1 << 32) for k in key):
-        raise ValueError("adamw8_step: key = %r (two 32-bit integers)" % (key,))
-    _step(True, params, grads, exp_avgs, exp_avg_sqs, scales, step, (int(key[0]), int(key[1])), lr, betas, eps, weight_decay, grad_scale,
-          copies, grad_mult, max_workgroups)
+    L.bind().adamw(True, params, grads, exp_avgs, exp_avg_sqs, scales, step, key, lr, betas, eps, weight_decay, grad_scale, copies, grad_mult,
+                   max_workgroups)
 
 
 # ---- the 8-bit states as tensors -----------------------------------------------------------------------------------------------------

@@ -335,3 +335,25 @@ def test_8_bit_rows_of_any_size():
         assert ((q.double() * s.double() - y).abs() <= y.abs() * (2.0 ** -4 + 2.0 ** -20) + s.double() * 2.0 ** -10 + 2.0 ** -149).all(), k
         if -100 <= k:
             assert torch.equal(q.float(), q0.float()), k
+
+
+def test_nothing_is_held_once_its_graph_is_gone():
+    from od_wscl_amd import layers
+    x, r, w = _rand(140, 64, 1000).requires_grad_(True), _rand(141, 64, 1000).requires_grad_(True), torch.ones(1000, device="cuda", requires_grad=True)
+
+    def once(back):
+        y, h = layers.rms_norm(x, w, residual=r)
+        if back:
+            torch.autograd.grad((y, h), (x, r, w), (y.detach(), h.detach()))
+    once(True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for k in range(20):
+        once(k % 2 == 0)
+    assert torch.cuda.memory_allocated() == before
+    y, h = layers.rms_norm(x, w, residual=r)
+    h.data.add_(0.0)                                     # (behind autograd's back)
+    with torch.no_grad():
+        h.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
