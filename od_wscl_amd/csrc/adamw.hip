@@ -3,11 +3,12 @@
 //
 // A launch takes up to kMaxTensors tensors (the norm kNormTensors): their pointers and sizes travel in the kernel's arguments (no table in device
 // memory to upload, nothing to keep alive for a captured launch).  The tensors are cut into chunks; a
-// workgroup finds the tensor of its chunk by bisection over the chunks' prefix -- the index is uniform, so this is scalar work.
+// workgroup finds the tensor of its chunk with one load of the chunks' prefix, a lane a tensor (the arguments lie in host memory: a bisection's six
+// dependent loads of them were half the time of a small launch).
 //
 // Both are bound by the bytes: an element's update is ~20 operations on 28 bytes with fp32 states (30 with a bf16 copy of p), ~70 on 16
 // (18) with 8-bit ones.  153 M parameters in 42 tensors with copies: 796 us (5.8 TB/s) and 463 us (5.9 TB/s); their gradients' norm
-// 88 us (7.0 TB/s), their scaling 220 us (5.5 TB/s).  A launch of a million elements takes 10-12 us.
+// 88 us (7.0 TB/s), their scaling 220 us (5.5 TB/s).  A launch of a million elements in 48 small tensors takes 8-10 us.
 #include "odw_common.h"
 #include "odw_rng.h"
 #include <math.h>
@@ -39,11 +40,11 @@ struct Tensor {
     uint64_t first;                      // the random counter of element 0
     float lr, wd;
     int flags;
-    int chunk0;                          // chunks of the tensors before this one
 };
 
 struct Args {
     Tensor t[kMaxTensors];
+    int chunk0[kMaxTensors];             // chunks of the tensors before each
     int count, chunks;
     float b1, b2, omb1, omb2, eps, c1, c2, mult;
     uint32_t k0, k1;
@@ -67,16 +68,28 @@ __device__ __forceinline__ unsigned short f2bf(float f) {      // round to neare
     return (unsigned short)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
 }
 
-// The tensor that chunk c lies in: the last one whose first chunk is not behind c.
-template <class F>
-__device__ __forceinline__ int find_tensor(F chunk0, int count, int c) {
-    int lo = 0, hi = count;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (chunk0(mid) <= c) lo = mid; else hi = mid;
+// The tensor that a chunk lies in, the last one whose first chunk is not behind it: lane l looks at tensors l, l + 64, ...
+template <int N>
+struct Prefix {
+    int first[(N + 63) / 64];
+    __device__ __forceinline__ Prefix(const int* chunk0, int count) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int k = 0; k < (N + 63) / 64; ++k) first[k] = lane + 64 * k < count ? chunk0[lane + 64 * k] : INT32_MAX;
     }
-    return lo;
-}
+    __device__ __forceinline__ int tensor_of(int c) const {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < (N + 63) / 64; ++k) n += __popcll(__ballot(first[k] <= c));
+        return n - 1;
+    }
+    __device__ __forceinline__ int chunk0_of(int t) const {
+        int x = __builtin_amdgcn_readlane(first[0], t & 63);
+#pragma unroll
+        for (int k = 1; k < (N + 63) / 64; ++k) x = t >= 64 * k ? __builtin_amdgcn_readlane(first[k], t & 63) : x;
+        return x;
+    }
+};
 
 // A wave's 256 elements, four consecutive ones a lane, by vectors declared with their element's alignment, which the memory instructions
 // take as well: tensors may start at any element.  Nothing is read twice: all loads and stores are marked nontemporal.
@@ -86,12 +99,12 @@ typedef f4 f4_any __attribute__((aligned(4)));
 typedef us4 us4_any __attribute__((aligned(2)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
 
-// `left` = elements from src on (FULL: at least 256 -- nothing to check).
+// `left` = elements from src on (FULL: at least 256 -- nothing to check; else it is the same for the whole wave, and may be negative).
 template <bool BF, bool FULL>
 struct Four {
     union { f4 f; us4 h; } u;
     __device__ __forceinline__ void load(const void* src, int lane, int left) {
-        if (FULL) {
+        if (FULL || left >= kBlock) {
             if (BF) u.h = __builtin_nontemporal_load((const us4_any*)src + lane);
             else u.f = __builtin_nontemporal_load((const f4_any*)src + lane);
         } else {
@@ -106,7 +119,7 @@ struct Four {
     __device__ __forceinline__ float get(int j) const { return BF ? bf2f(u.h[j]) : u.f[j]; }
     __device__ __forceinline__ void set(int j, float x) { if (BF) u.h[j] = f2bf(x); else u.f[j] = x; }
     __device__ __forceinline__ void store(void* dst, int lane, int left) const {
-        if (FULL) {
+        if (FULL || left >= kBlock) {
             if (BF) __builtin_nontemporal_store(u.h, (us4_any*)dst + lane);
             else __builtin_nontemporal_store(u.f, (f4_any*)dst + lane);
         } else {
@@ -123,7 +136,7 @@ struct Four {
 
 template <bool FULL>
 __device__ __forceinline__ uint32_t load_codes(const uint8_t* src, int lane, int left) {
-    if (FULL) return __builtin_nontemporal_load((const u32_any*)src + lane);
+    if (FULL || left >= kBlock) return __builtin_nontemporal_load((const u32_any*)src + lane);
     uint32_t u = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -133,7 +146,7 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* src, int lane, int
 
 template <bool FULL>
 __device__ __forceinline__ void store_codes(uint8_t* dst, int lane, int left, uint32_t u) {
-    if (FULL) {
+    if (FULL || left >= kBlock) {
         __builtin_nontemporal_store(u, (u32_any*)dst + lane);
         return;
     }
@@ -192,12 +205,12 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 
 struct Step { float gs, rc2, step, decay; uint32_t k1; };
 
-// p, g, m, v in, p, m, v (and p's bf16 copy) out, for U blocks of 256 elements `stride` apart: all loads first.  The averages are formed with
+// p, g, m, v in, p, m, v (and p's bf16 copy) out, for U blocks of 256 elements `stride` apart, `left0` elements being there from the first one's start: all loads first.  The averages are formed with
 // one rounding an operation (no contraction), in the order m b1 + g (1 - b1), v b2 + g g (1 - b2); the ratio with the hardware's root and
 // reciprocal (1 ulp each: 2^-22 of a step of lr is far below p's rounding; eps keeps the reciprocal's argument above 1e-15 and makes roots
 // of subnormal numbers, which the instruction takes for zero, irrelevant).
 template <bool BITS8, bool PBF, bool GBF, bool FULL, int U>
-__device__ __forceinline__ void update(const Args& a, const Tensor& t, const Step& s, int64_t base, int64_t stride, int lane, int left) {
+__device__ __forceinline__ void update(const Args& a, const Tensor& t, const Step& s, int64_t base, int stride, int lane, int left0) {
     Four<PBF, FULL> p[U];
     Four<GBF, FULL> g[U];
     Four<false, FULL> fm[U], fv[U];
@@ -205,6 +218,8 @@ __device__ __forceinline__ void update(const Args& a, const Tensor& t, const Ste
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int64_t o = base + u * stride;
+        const int left = left0 - u * stride;
+        if (!FULL && left <= 0) continue;
         p[u].load((const char*)t.p + o * (PBF ? 2 : 4), lane, left);
         g[u].load((const char*)t.g + o * (GBF ? 2 : 4), lane, left);
         if (BITS8) {
@@ -219,6 +234,8 @@ __device__ __forceinline__ void update(const Args& a, const Tensor& t, const Ste
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int64_t o = base + u * stride;
+        const int left = left0 - u * stride;
+        if (!FULL && left <= 0) continue;
         float m[4], v[4];
         if (BITS8) {
             const float sm = __uint_as_float((ee[u] & 0xFFu) << 23), sv = __uint_as_float((ee[u] >> 16) << 23);
@@ -276,19 +293,14 @@ __device__ __forceinline__ void update(const Args& a, const Tensor& t, const Ste
     }
 }
 
-// A chunk: its four waves take every fourth block, all at once where the chunk is a whole one; the tensor's last, short block by itself.
+// A chunk: its four waves take every fourth block, all at once -- a tensor's last, short chunk as well, whose blocks one after the other would
+// cost small tensors a round trip to memory each.
 template <bool BITS8, bool PBF, bool GBF>
 __device__ __forceinline__ void chunk(const Args& a, const Tensor& t, const Step& s, int64_t begin, int wave, int lane) {
-    const int64_t rest = t.n - begin;
-    constexpr int kChunk = chunk_of(BITS8), kUnroll = unroll(BITS8), kWaves = kThreads / 64;
-    const int size = rest < kChunk ? (int)rest : kChunk, blocks = size / kBlock;
-    int b = wave;
-    if (blocks == kUnroll * kWaves) {
-        update<BITS8, PBF, GBF, true, kUnroll>(a, t, s, begin + b * kBlock, kWaves * kBlock, lane, kBlock);
-        return;
-    }
-    for (; b < blocks; b += kWaves) update<BITS8, PBF, GBF, true, 1>(a, t, s, begin + b * kBlock, 0, lane, kBlock);
-    if (b == blocks && size % kBlock) update<BITS8, PBF, GBF, false, 1>(a, t, s, begin + b * kBlock, 0, lane, size % kBlock);
+    constexpr int kWaves = kThreads / 64;
+    const int64_t rest = t.n - begin, base = begin + wave * kBlock;
+    if (rest >= chunk_of(BITS8)) update<BITS8, PBF, GBF, true, unroll(BITS8)>(a, t, s, base, kWaves * kBlock, lane, 0);
+    else update<BITS8, PBF, GBF, false, unroll(BITS8)>(a, t, s, base, kWaves * kBlock, lane, (int)rest - wave * kBlock);
 }
 
 template <bool BITS8>
@@ -304,10 +316,11 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Args a) {
     }
     s.gs = a.scale ? a.mult * *a.scale : a.mult;
     s.rc2 = 1.0f / sqrtf(c2);
+    const Prefix<kMaxTensors> prefix(a.chunk0, a.count);
     for (int c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-        const int ti = find_tensor([&](int i) { return a.t[i].chunk0; }, a.count, c);
+        const int ti = prefix.tensor_of(c);
         const Tensor& t = a.t[ti];
-        const int64_t begin = (int64_t)(c - t.chunk0) * chunk_of(BITS8);
+        const int64_t begin = (int64_t)(c - prefix.chunk0_of(ti)) * chunk_of(BITS8);
         s.step = t.lr / c1;
         s.decay = t.lr * t.wd;
         switch (t.flags) {                         // (a tensor's types: uniform)
@@ -345,11 +358,14 @@ __device__ __forceinline__ double sqsum(const void* g, int size, int wave, int l
 #pragma unroll
             for (int j = 0; j < 4; ++j) s = fma((double)x[u].get(j), (double)x[u].get(j), s);
     }
-    for (; b * kBlock < size; b += kWaves) {
-        Four<BF, false> x;
-        x.load((const char*)g + (size_t)b * kBlock * (BF ? 2 : 4), lane, size - b * kBlock);
+    for (; b * kBlock < size; b += U * kWaves) {
+        Four<BF, false> x[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s = fma((double)x.get(j), (double)x.get(j), s);
+        for (int u = 0; u < U; ++u) x[u].load((const char*)g + (size_t)(b + u * kWaves) * kBlock * (BF ? 2 : 4), lane, size - (b + u * kWaves) * kBlock);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s = fma((double)x[u].get(j), (double)x[u].get(j), s);
     }
     return s;
 }
@@ -358,8 +374,9 @@ __global__ __launch_bounds__(kThreads) void sqsum_kernel(const NormArgs a, doubl
     __shared__ double part[kThreads / 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = blockIdx.x;
-    const int ti = find_tensor([&](int i) { return a.chunk0[i]; }, a.count, c);
-    const int64_t begin = (int64_t)(c - a.chunk0[ti]) * kNormChunk, rest = a.n[ti] - begin;
+    const Prefix<kNormTensors> prefix(a.chunk0, a.count);
+    const int ti = prefix.tensor_of(c);
+    const int64_t begin = (int64_t)(c - prefix.chunk0_of(ti)) * kNormChunk, rest = a.n[ti] - begin;
     const int size = rest < kNormChunk ? (int)rest : kNormChunk;
     const bool bf = a.flags[ti] & kGBf16;
     const char* g = (const char*)a.g[ti] + begin * (bf ? 2 : 4);
@@ -421,8 +438,9 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(const NormArgs a, const
     if (s == 1.0f) return;                       // the products would be what is there
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = blockIdx.x;
-    const int ti = find_tensor([&](int i) { return a.chunk0[i]; }, a.count, c);
-    const int64_t begin = (int64_t)(c - a.chunk0[ti]) * kNormChunk, rest = a.n[ti] - begin;
+    const Prefix<kNormTensors> prefix(a.chunk0, a.count);
+    const int ti = prefix.tensor_of(c);
+    const int64_t begin = (int64_t)(c - prefix.chunk0_of(ti)) * kNormChunk, rest = a.n[ti] - begin;
     const int size = rest < kNormChunk ? (int)rest : kNormChunk;
     const bool bf = a.flags[ti] & kGBf16;
     char* g = (char*)const_cast<void*>(a.g[ti]) + begin * (bf ? 2 : 4);
@@ -493,12 +511,12 @@ int adamw(bool bits8, int n_tensors, void* const* p, const void* const* g, void*
         for (; i < n_tensors && a.count < kMaxTensors; ++i) {
             if (n[i] == 0) continue;
             if (a.count && a.chunks + chunks_of(n[i], chunk_of(bits8)) > INT32_MAX) break;
+            a.chunk0[a.count] = a.chunks;
             Tensor& t = a.t[a.count++];
             t.p = p[i]; t.g = g[i]; t.m = m[i]; t.v = v[i]; t.e = bits8 ? e[i] : nullptr;
             t.copy = copy ? (unsigned short*)copy[i] : nullptr;
             t.n = n[i]; t.first = first; t.lr = lr[i]; t.wd = wd[i];
             t.flags = types[i];
-            t.chunk0 = a.chunks;
             a.chunks += (int)chunks_of(n[i], chunk_of(bits8));
             first += (uint64_t)n[i];
         }
