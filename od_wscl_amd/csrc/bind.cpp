@@ -159,7 +159,7 @@ std::vector<float> scalars(const char* what, const char* name, const py::object&
     std::vector<float> out;
     out.reserve(n);
     auto push = [&](double x) {
-        if (!(x >= 0.0 && std::isfinite(x))) value_error("%s: %s = %g", what, name, x);
+        if (!(x >= 0.0 && std::isfinite((float)x))) value_error("%s: %s = %g", what, name, x);
         out.push_back((float)x);
     };
     if (PyFloat_Check(value.ptr()) || PyLong_Check(value.ptr())) {
@@ -215,8 +215,8 @@ void adamw(bool bits8, const std::vector<Tensor>& params, const std::vector<Tens
     }
     if (betas.size() != 2 || !(betas[0] >= 0.0 && betas[0] < 1.0) || !(betas[1] >= 0.0 && betas[1] < 1.0)) value_error("%s: betas have to be two numbers in [0, 1)", what);
     // (a gradient whose square is nothing in fp32, below 1e-21, then moves p by at most lr * 1e-6, not by lr * g / eps of any size)
-    if (!(eps >= 1e-15 && std::isfinite(eps))) value_error("%s: eps = %g", what, eps);
-    if (!std::isfinite(grad_mult)) value_error("%s: grad_mult = %g", what, grad_mult);
+    if (!(eps >= 1e-15 && std::isfinite((float)eps))) value_error("%s: eps = %g", what, eps);
+    if (!std::isfinite((float)grad_mult)) value_error("%s: grad_mult = %g", what, grad_mult);
     const std::vector<float> lrs = scalars(what, "lr", lr, count), wds = scalars(what, "weight_decay", weight_decay, count);
     if (grad_scale) device_scalar(what, "grad_scale", *grad_scale, device, at::kFloat);
     std::vector<int> types;
@@ -283,7 +283,7 @@ void check_rows(const char* what, const Tensor& x, const OptTensor& weight, cons
     if (residual && residual->sizes() != x.sizes()) value_error("%s: residual has another shape than x", what);
     if (residual && residual->scalar_type() != x.scalar_type() && residual->scalar_type() != at::kFloat)
         type_error("%s: residual is %s beside x in %s (x's type or torch.float32)", what, name_of(residual->scalar_type()).c_str(), name_of(x.scalar_type()).c_str());
-    if (!(eps >= 0.0 && std::isfinite(eps))) value_error("%s: eps = %g", what, eps);
+    if (!(eps >= 0.0 && std::isfinite((float)eps))) value_error("%s: eps = %g", what, eps);
 }
 
 int types_of(at::ScalarType x, at::ScalarType h, const Tensor& w) { return is_bf16(x) + 2 * is_bf16(h) + (w.defined() && is_bf16(w.scalar_type()) ? 4 : 0); }

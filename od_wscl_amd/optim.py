@@ -13,6 +13,7 @@ counter-based stream of utils/rng.py -- a step is a function of its inputs and i
 
 Every tensor is on one GPU; the work goes to the current stream of that device; nothing is read back to the host."""
 import math
+from collections import defaultdict
 
 import torch
 
@@ -20,21 +21,26 @@ from . import _lib as L
 from .utils import rng
 
 BLOCK = 256          # elements that share a scale of the 8-bit states
+STATE8 = {"exp_avg": torch.float8_e4m3fn, "exp_avg_sq": torch.float8_e5m2}
 MIN_EPS = 1e-15      # (a smaller eps is refused: csrc/bind.cpp says why)
 
 
+def _list(grads):
+    return [grads] if torch.is_tensor(grads) else list(grads)          # (iterating over one parameter would give rows of its values)
+
+
 def grad_norm(grads, max_norm=None):
-    """The 2-norm over all of `grads` (tensors, or parameters that stand for their .grad) as a 0-dim fp32 tensor; summed in fp64 in
+    """The 2-norm over all of `grads` (tensors, or parameters that stand for their .grad; or one) as a 0-dim fp32 tensor; summed in fp64 in
     one order, so the same from run to run.  With max_norm: (norm, coef), coef = min(1, max_norm / (norm + 1e-6)) -- the factor
     that clips them, for `grad_scale` of adamw_step (clipping without a pass over the gradients).  Neither is read by the host.
     A non-finite gradient makes the norm inf or NaN, and coef 0 or NaN."""
-    return L.bind().grad_norm(list(grads), max_norm)
+    return L.bind().grad_norm(_list(grads), max_norm)
 
 
 def clip_grad_norm_(grads, max_norm):
-    """Scale all of `grads` (tensors, or parameters that stand for their .grad) in place so that their common 2-norm is at most
+    """Scale all of `grads` (tensors, or parameters that stand for their .grad; or one) in place so that their common 2-norm is at most
     max_norm; returns the norm before that (torch.nn.utils.clip_grad_norm_, without a host read)."""
-    return L.bind().clip_grad_norm(list(grads), max_norm)
+    return L.bind().clip_grad_norm(_list(grads), max_norm)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, grad_scale=None,
@@ -132,6 +138,20 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm = None            # of the last step, where it was clipped (0-dim, on the GPU)
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    # Copies and pickles: the base class keeps its own attributes only, and a plain pickle knows no 8-bit floats (they go as bytes).
+    def __getstate__(self):
+        own = ("state_bits", "max_grad_norm", "seed", "capturable", "grad_norm")
+        data = dict(super().__getstate__(), **{k: self.__dict__[k] for k in own})
+        if self.state_bits == 8:
+            data["state"] = defaultdict(dict, {p: dict(st, **{k: st[k].view(torch.uint8) for k in STATE8}) for p, st in self.state.items()})
+        return data
+
+    def __setstate__(self, data):
+        super().__setstate__(data)
+        if self.state_bits == 8:
+            for st in self.state.values():
+                st.update({k: st[k].view(t) for k, t in STATE8.items()})
+
     def _state(self, p):
         st = self.state[p]
         if not st:
@@ -215,7 +235,11 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
-        """A state_dict() of this class (of either state_bits) or of torch.optim.AdamW."""
+        """A state_dict() of this class (of either state_bits) or of torch.optim.AdamW (without amsgrad and maximize)."""
+        for g in state_dict["param_groups"]:
+            other = [k for k in ("amsgrad", "maximize") if g.get(k)] + ["coupled weight decay"] * (not g.get("decoupled_weight_decay", True))
+            if other:
+                raise ValueError("AdamW: the state is of an optimiser with %s" % ", ".join(other))
         states = dict(state_dict["state"])
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         shared = {}

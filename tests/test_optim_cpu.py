@@ -1,6 +1,8 @@
 """Argument checks of the optimiser's and the row norm's entry points that end before any launch, and the 8-bit states' layout, without a GPU."""
+import copy
 import ctypes
 import math
+import pickle
 
 import pytest
 import torch
@@ -35,6 +37,41 @@ def test_optimiser_arguments():
                 dict(betas=(0.9, 1.0)), dict(eps=0.0), dict(eps=math.inf)):
         with pytest.raises(ValueError):
             optim.AdamW(p, **bad)
+
+
+def _with_a_state(**more):
+    p = torch.nn.Parameter(torch.arange(6.0))
+    opt = optim.AdamW([p], lr=2e-3, **more)
+    src = torch.optim.AdamW([p], lr=3e-3, weight_decay=0.1)
+    p.grad = torch.linspace(-1.0, 1.0, 6)
+    src.step()
+    opt.load_state_dict(src.state_dict())
+    return opt
+
+
+@pytest.mark.parametrize("way", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))], ids=["copy", "pickle"])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_copied_optimiser_is_whole(way, bits):
+    opt = _with_a_state(state_bits=bits, max_grad_norm=2.0, seed=7)
+    got = way(opt)
+    assert (got.state_bits, got.max_grad_norm, got.seed, got.capturable, got.grad_norm) == (bits, 2.0, 7, False, None)
+    a, b = opt.state_dict(), got.state_dict()
+    assert a["param_groups"] == b["param_groups"] and a["state"].keys() == b["state"].keys()
+    for i in a["state"]:
+        for k in ("step", "exp_avg", "exp_avg_sq"):
+            assert torch.equal(a["state"][i][k], b["state"][i][k])
+    with pytest.raises(RuntimeError, match="not on the GPU"):
+        got.param_groups[0]["params"][0].grad = torch.ones(6)
+        got.step()
+
+
+def test_states_of_another_rule_are_refused():
+    p = torch.nn.Parameter(torch.zeros(4))
+    opt = optim.AdamW([p])
+    for other in (torch.optim.AdamW([p], amsgrad=True), torch.optim.AdamW([p], maximize=True), torch.optim.Adam([p], weight_decay=0.1)):
+        with pytest.raises(ValueError, match="amsgrad|maximize|coupled"):
+            opt.load_state_dict(other.state_dict())
+    opt.load_state_dict(torch.optim.AdamW([p]).state_dict())
 
 
 def test_library_checks_come_before_launches():

@@ -1,5 +1,6 @@
 """csrc/adamw.hip through optim.adamw_step / adamw8_step / grad_norm / clip_grad_norm_ / AdamW: the update against its formula in 64 bits,
 the 8-bit codes bit for bit against their definition."""
+import copy
 import math
 
 import numpy as np
@@ -573,3 +574,46 @@ def test_tensors_made_in_inference_mode():
         optim.clip_grad_norm_([g], 1.0)
         y, h = layers.rms_norm(p.view(3, 100), g[:100], residual=v.view(3, 100))
     assert (p < 1).all() and abs(g.norm().item() - 1) < 1e-5 and torch.isfinite(y).all()
+
+
+def test_one_parameter_stands_for_its_gradient():
+    from od_wscl_amd import optim
+    p = torch.nn.Parameter(torch.full((6, 5), 3.0, device="cuda"))
+    p.grad = torch.full((6, 5), 2.0, device="cuda")
+    want = math.sqrt(30 * 4.0)                                     # (a sum of small integers: exact; its root rounded once)
+    assert float(optim.grad_norm(p)) == torch.tensor(want).item() == float(optim.grad_norm([p]))
+    assert float(optim.clip_grad_norm_(p, 1e3)) == torch.tensor(want).item()
+    assert torch.equal(p.grad, torch.full_like(p, 2.0)) and torch.equal(p.detach(), torch.full_like(p, 3.0))
+
+
+def test_numbers_past_fp32_are_refused():
+    from od_wscl_amd import layers, optim
+    t = [torch.ones(4, device="cuda") for _ in range(4)]
+    args = [[x] for x in t]
+    for more in (dict(lr=1e39), dict(lr=[1e39]), dict(weight_decay=1e39), dict(eps=1e39), dict(grad_mult=1e39), dict(grad_mult=-1e39)):
+        with pytest.raises(ValueError):
+            optim.adamw_step(*args, 1, **more)
+    for x in t:
+        assert torch.equal(x, torch.ones_like(x))
+    with pytest.raises(ValueError, match="eps"):
+        layers.rms_norm(torch.ones(2, 4, device="cuda"), eps=1e39)
+
+
+@pytest.mark.parametrize("bits,capturable", [(32, False), (8, False), (8, True)])
+def test_a_copied_optimiser_goes_on_alike(bits, capturable):
+    from od_wscl_amd import optim
+    torch.manual_seed(5)
+    mod = torch.nn.Linear(37, 19).cuda()
+    opt = optim.AdamW(mod.parameters(), state_bits=bits, capturable=capturable, max_grad_norm=0.5, seed=3)
+
+    def step(m, o, k):
+        for i, p in enumerate(m.parameters()):
+            p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(10 * k + i)).cuda()
+        o.step()
+    step(mod, opt, 1)
+    twin, topt = copy.deepcopy((mod, opt))
+    for k in (2, 3):
+        step(mod, opt, k)
+        step(twin, topt, k)
+    for a, b in zip(mod.parameters(), twin.parameters()):
+        assert a is not b and torch.equal(a, b)
