@@ -657,8 +657,10 @@ class FlatAdamW(FlatSGD):
         return {"state": state, "param_groups": groups}
 
     def load_state_dict(self, model, sd):
-        """Averages and step count of a checkpoint written by state_dict() above (with either STATE_BITS) or by torch.optim.AdamW."""
+        """Averages and step count of a checkpoint written by state_dict() above (with either STATE_BITS) or by torch.optim.AdamW (without
+        amsgrad and maximize)."""
         from . import optim
+        optim.refuse_other_rules(sd.get("param_groups", []))
         self.join_side()
         order = self._param_order(model)
         state = sd.get("state", {})

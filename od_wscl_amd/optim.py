@@ -111,6 +111,14 @@ def state8_write(m, v, out=None):
 # ---- the optimiser object ------------------------------------------------------------------------------------------------------------
 
 
+def refuse_other_rules(param_groups):
+    """Groups of a torch optimiser whose averages mean, or whose steps did, something else than adamw_step's."""
+    for g in param_groups:
+        other = [k for k in ("amsgrad", "maximize") if g.get(k)] + ["coupled weight decay"] * (not g.get("decoupled_weight_decay", True))
+        if other:
+            raise ValueError("AdamW: the state is of an optimiser with %s" % ", ".join(other))
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's arguments, groups and state names on the kernels above.
 
@@ -236,10 +244,7 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """A state_dict() of this class (of either state_bits) or of torch.optim.AdamW (without amsgrad and maximize)."""
-        for g in state_dict["param_groups"]:
-            other = [k for k in ("amsgrad", "maximize") if g.get(k)] + ["coupled weight decay"] * (not g.get("decoupled_weight_decay", True))
-            if other:
-                raise ValueError("AdamW: the state is of an optimiser with %s" % ", ".join(other))
+        refuse_other_rules(state_dict["param_groups"])
         states = dict(state_dict["state"])
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         shared = {}

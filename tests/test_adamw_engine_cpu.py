@@ -94,3 +94,13 @@ def test_schedule_does_not_touch_the_averages():
     o.set_iteration(4)
     o.set_iteration(5)                                          # SGD rescales its momentum at this jump of 10
     assert abs(o.lr_scale - 0.1) < 1e-12 and (o.flat_m == 1).all()
+
+
+def test_states_of_another_rule_are_refused():
+    from od_wscl_amd import engine
+    net = Net()
+    groups = [{"params": [p]} for p in net.parameters() if p.requires_grad]
+    o = engine.build_optimizer(_cfg(), net)
+    for other in (torch.optim.AdamW(groups, amsgrad=True), torch.optim.AdamW(groups, maximize=True), torch.optim.Adam(groups, weight_decay=0.1)):
+        with pytest.raises(ValueError, match="amsgrad|maximize|coupled"):
+            o.load_state_dict(net, other.state_dict())
