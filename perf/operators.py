@@ -10,11 +10,8 @@ its 8-bit output), and the AdamW update of many tensors at once (states in 32 or
             p -= lr (m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps) + weight_decay p)
     adamw8  the same with m and v held between steps as 8-bit floats (float8_e4m3fn and float8_e5m2), one power-of-two scale each
             for 256 consecutive elements of a tensor, rounded stochastically: a value between two neighbours of the format goes to
-            the upper one with the probability of its distance from the lower one; only a v that is not zero never becomes zero
-            (at least 2^-16 of its scale, the format's smallest number: a root of zero would make the next update of what the
-            rounding left of m).  Random bits: 16 a value from the package's counter-based stream, element counter = position
-            in the concatenation of the tensors; the stream's second key is key[1] + 0x9E3779B9 key[0], so that steps whose
-            keys differ in the first word alone do not draw from one set of numbers.
+            the upper one with the probability of its distance from the lower one.  Random bits: 16 a value from the package's
+            counter-based stream, element counter = position in the concatenation of the tensors.
 
 The scale of a block with largest magnitude a: 2^(floor(log2 a) - k), twice that where a's mantissa is over 1.75 (k = 8 for m, 15 for
 v: the formats' largest values are 1.75 * 2^8 and 1.75 * 2^15); held as its exponent + 127, between 1 and 254.
@@ -198,10 +195,7 @@ def prepare(case, seed):
                 x = torch.nn.functional.pad(flat[o:o + n], (0, -n % BLOCK)).view(-1, BLOCK)
                 b = block_exponents(x.abs().amax(1), k)
                 e[:, col] = b.to(torch.uint8)
-                y = (x * ((254 - b) << 23).view(torch.float32).view(-1, 1)).view(-1)[:n]
-                if col == 1:
-                    y = torch.where(x.view(-1)[:n] > 0, y.clamp_min(2.0 ** -16), y)
-                q = y.to(out.dtype)
+                q = torch.ldexp(x, 127 - b.view(-1, 1)).view(-1)[:n].to(out.dtype)
                 out.view(torch.uint8)[o:o + n] = q.view(torch.uint8)
         s["m"] = [s["flat_m"].view(torch.uint8)[o:o + n].view(torch.float8_e4m3fn) for o, n in zip(at, sizes)]
         s["v"] = [s["flat_v"].view(torch.uint8)[o:o + n].view(torch.float8_e5m2) for o, n in zip(at, sizes)]
@@ -258,22 +252,21 @@ def plain_mix(x):
 def plain_bits(first, n, key):
     i = torch.arange(first, first + n, device="cuda")
     h = plain_mix((i & 0xFFFFFFFF) ^ key[0])
-    return plain_mix((h + key[1] + 0x9E3779B9 * key[0] + (i >> 32)) & 0xFFFFFFFF)
+    return plain_mix((h + key[1] + (i >> 32)) & 0xFFFFFFFF)
 
 
-def plain_encode(x, rand, k, bias, mantissa, least):
+def plain_encode(x, rand, k, bias, mantissa):
     """fp32 values and 16 random bits each -> (codes as uint8, the blocks' exponents): the bits below the format's last mantissa bit
-    take a random number's addition and are cut; below the smallest normal number, 2^(1 - bias), the same of the value in fixed
-    point.  `least`: the smallest code of a value that is not zero."""
+    take a random number's addition and are cut; below the smallest normal number the values are moved up by it first, where the
+    format's steps are the same."""
     n = x.numel()
     blocks = torch.nn.functional.pad(x.abs(), (0, -n % BLOCK)).view(-1, BLOCK)
     e = block_exponents(blocks.amax(1), k)
     y = (blocks * ((254 - e) << 23).view(torch.float32).view(-1, 1)).view(-1)[:n]
     low = y < 2.0 ** (1 - bias)
     drop = 23 - mantissa
-    word = torch.where(low, (y * 2.0 ** (22 + bias)).to(torch.int32), y.view(torch.int32) - ((127 - bias) << 23))
-    code = (word + ((rand << (drop - 16)) + (1 << (drop - 17))).to(torch.int32)) >> drop
-    code = torch.where(x != 0, code.clamp_min(least), code)
+    z = torch.where(low, y + 2.0 ** (1 - bias), y).view(torch.int32) + ((rand << (drop - 16)) + (1 << (drop - 17))).to(torch.int32)
+    code = (z >> drop) - ((127 - bias) << mantissa) - (low.to(torch.int32) << mantissa)
     return (code | (torch.signbit(x).to(torch.int32) << 7)).to(torch.uint8), e.to(torch.uint8)
 
 
@@ -286,9 +279,9 @@ def plain_adamw8(p, g, mq, vq, e, first, key, c1, c2):
     m, v = plain_averages(g.float(), plain_decode(mq, e[:, 0]), plain_decode(vq, e[:, 1]))
     p.copy_(plain_update(p, m, v, c1, c2))
     bits = plain_bits(first, p.numel(), key)
-    code, em = plain_encode(m, bits & 0xFFFF, 8, 7, 3, 0)
+    code, em = plain_encode(m, bits & 0xFFFF, 8, 7, 3)
     mq.view(torch.uint8).copy_(code)
-    code, ev = plain_encode(v, bits >> 16, 15, 15, 2, 1)
+    code, ev = plain_encode(v, bits >> 16, 15, 15, 2)
     vq.view(torch.uint8).copy_(code)
     e.copy_(torch.stack([em, ev], 1))
 
@@ -412,14 +405,13 @@ def work(case):
 # ---- the definitions in 64 bits --------------------------------------------------------------------------------------------------
 
 
-def exact_round8(x, scale_exp, frac, digits, lowest, least):
+def exact_round8(x, scale_exp, frac, digits, lowest):
     """x (64 bits) on the grid of an 8-bit float: steps of 2^(e - digits) for x in [2^e, 2^(e+1)), e not under `lowest`; up where
-    the distance from the lower neighbour, in steps, is more than 1 - frac; numbers but zero are at least `least`."""
+    the distance from the lower neighbour, in steps, is more than 1 - frac."""
     y = torch.ldexp(x.abs(), -scale_exp)
     e = (torch.frexp(y)[1] - 1).clamp_min(lowest)
     steps = torch.ldexp(y, digits - e)
-    near = torch.ldexp(torch.floor(steps + frac), e - digits)
-    return torch.copysign(torch.where(x == 0, near, near.clamp_min(least)), x)
+    return torch.copysign(torch.ldexp(torch.floor(steps + frac), e - digits), x)
 
 
 def exact_scale(x, k):
@@ -441,7 +433,7 @@ def exact_random(first, n, key):
             a, b = w // 65536, w % 65536                        # 32-bit product in two halves
             w = ((a * factor % 65536) * 65536 + b * factor) % (1 << 32)
         return w
-    w = scramble((scramble(torch.bitwise_xor(low, torch.full_like(low, key[0]))) + (key[1] + key[0] * 0x9E3779B9) % (1 << 32) + high) % (1 << 32))
+    w = scramble((scramble(torch.bitwise_xor(low, torch.full_like(low, key[0]))) + key[1] + high) % (1 << 32))
     return (w % 65536 + 0.5).double() / 65536, (w // 65536 + 0.5).double() / 65536
 
 
@@ -507,7 +499,7 @@ def exact(case, seed):
                 out["copy"][o:o + n] = p
             if case["op"] == "adamw8":
                 rm, rv = exact_random(first, n, key_of(s["seed"], t))
-                m.copy_(exact_round8(m, exact_scale(m, 8), rm, 3, -6, 0.0))
-                v.copy_(exact_round8(v, exact_scale(v, 15), rv, 2, -14, 2.0 ** -16))
+                m.copy_(exact_round8(m, exact_scale(m, 8), rm, 3, -6))
+                v.copy_(exact_round8(v, exact_scale(v, 15), rv, 2, -14))
             first += n
         return out
