@@ -712,7 +712,8 @@ int odw_adamw(int n_tensors, void* const* p, const void* const* g, void* const* 
 /* The same with 8-bit states: m = float8 e4m3 (OCP, no infinity), v = float8 e5m2 codes of n[i] bytes, e[i] = 2 bytes for each 256
  * elements of the tensor: exponent + 127 of the power-of-two scales of m and v.  Rounded stochastically with 16 bits a value of the
  * counter-based stream (k0, k1 + 0x9E3779B9 k0); the counter of an element is its position in the concatenation of the list's tensors (with
- * bias != NULL the step is added to k1).  Non-finite averages become NaN codes. */
+ * bias != NULL the step is added to k1).  Non-finite averages become NaN codes.  A v that is not zero is held as 2^-16 of its scale at
+ * least; types[i] bit 2 = v is rounded to zero like any other value. */
 int odw_adamw8(int n_tensors, void* const* p, const void* const* g, void* const* m, void* const* v, uint8_t* const* e,
                void* const* copy, const int64_t* n, const int* types, const float* lr, const float* wd, double beta1, double beta2,
                double eps, int64_t step, const float* bias, const float* grad_scale, float grad_mult, uint32_t k0, uint32_t k1,

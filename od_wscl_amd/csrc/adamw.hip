@@ -27,7 +27,7 @@ constexpr int kMaxGrid = 1 << 23;        // (a launch has fewer than 2^32 thread
 constexpr int kNormChunk = 16384;        // the same of the norm: fewer partial sums for the workgroup that adds them
 constexpr int kThreads = 256;
 
-enum { kPBf16 = 1, kGBf16 = 2 };
+enum { kPBf16 = 1, kGBf16 = 2, kVToZero = 4 };
 
 struct Tensor {
     void* p;
@@ -165,10 +165,11 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, int lane, int left, ui
 // a bias of v, instead of one larger than v itself.
 // A v that is not zero is held as 2^-16 of its scale at least.  An element whose gradients are far below its block's largest can have
 // its m rounded up to the smallest number, 2^-17 of the block's largest m; over a v held as zero that would be an update of any size
-// -- over 2^-32 of the block's largest v it is at most lr x a few (largest m <= 3.2 sqrt(largest v) for beta = 0.9, 0.999).
+// -- over 2^-32 of the block's largest v it is at most lr x a few (largest m <= 3.2 sqrt(largest v) for beta = 0.9, 0.999).  (kVToZero: v is
+// rounded to zero like any other value, without that bound.)
 // All of it is integer arithmetic on the fp32 words: the same bits whatever the launch geometry.
-template <int BIAS, int MANT, uint32_t LEAST>
-__device__ __forceinline__ uint32_t encode8(float x, float inv_scale, uint32_t rand16, bool any_bad) {
+template <int BIAS, int MANT>
+__device__ __forceinline__ uint32_t encode8(float x, float inv_scale, uint32_t rand16, uint32_t least, bool any_bad) {
     constexpr int kDrop = 23 - MANT;
     const float y = fabsf(x) * inv_scale;
     const uint32_t u = __float_as_uint(y);
@@ -177,7 +178,7 @@ __device__ __forceinline__ uint32_t encode8(float x, float inv_scale, uint32_t r
     const uint32_t word = u < ((uint32_t)(128 - BIAS) << 23) ? (uint32_t)(y * __uint_as_float((uint32_t)(149 + BIAS) << 23))
                                                              : u - ((uint32_t)(127 - BIAS) << 23);
     uint32_t code = (word + (rand16 << (kDrop - 16)) + (1u << (kDrop - 17))) >> kDrop;
-    if (code < LEAST && x != 0.0f) code = LEAST;
+    if (code < least && x != 0.0f) code = least;
     if (any_bad && (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u) code = 0x7Fu;
     return code | ((__float_as_uint(x) >> 31) << 7);
 }
@@ -203,7 +204,7 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
     return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-struct Step { float gs, rc2, step, decay; uint32_t k1; };
+struct Step { float gs, rc2, step, decay; uint32_t k1, least_v; };
 
 // p, g, m, v in, p, m, v (and p's bf16 copy) out, for U blocks of 256 elements `stride` apart, `left0` elements being there from the first one's start: all loads first.  The averages are formed with
 // one rounding an operation (no contraction), in the order m b1 + g (1 - b1), v b2 + g g (1 - b2); the ratio with the hardware's root and
@@ -281,8 +282,8 @@ __device__ __forceinline__ void update(const Args& a, const Tensor& t, const Ste
         for (int j = 0; j < 4; ++j) {
             const uint64_t c = t.first + (uint64_t)o + (uint64_t)(4 * lane + j);
             const uint32_t r = odw_mix(odw_mix((uint32_t)c ^ a.k0) + s.k1 + (uint32_t)(c >> 32));
-            om |= encode8<7, 3, 0>(m[j], im, r & 0xFFFFu, bad) << (8 * j);
-            ov |= encode8<15, 2, 1>(v[j], iv, r >> 16, bad) << (8 * j);
+            om |= encode8<7, 3>(m[j], im, r & 0xFFFFu, 0, bad) << (8 * j);
+            ov |= encode8<15, 2>(v[j], iv, r >> 16, s.least_v, bad) << (8 * j);
         }
         store_codes<FULL>((uint8_t*)t.m + o, lane, left, om);
         store_codes<FULL>((uint8_t*)t.v + o, lane, left, ov);
@@ -323,7 +324,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Args a) {
         const int64_t begin = (int64_t)(c - prefix.chunk0_of(ti)) * chunk_of(BITS8);
         s.step = t.lr / c1;
         s.decay = t.lr * t.wd;
-        switch (t.flags) {                         // (a tensor's types: uniform)
+        s.least_v = t.flags & kVToZero ? 0 : 1;
+        switch (t.flags & (kPBf16 | kGBf16)) {     // (a tensor's types: uniform)
             case 0: chunk<BITS8, false, false>(a, t, s, begin, wave, lane); break;
             case kPBf16: chunk<BITS8, true, false>(a, t, s, begin, wave, lane); break;
             case kGBf16: chunk<BITS8, false, true>(a, t, s, begin, wave, lane); break;
@@ -468,12 +470,12 @@ int fill_norm_args(NormArgs& a, int i, int n_tensors, const void* const* g, cons
     return i;
 }
 
-int check_list(const char* what, int n_tensors, const void* const* g, const int64_t* n, const int* types) {
+int check_list(const char* what, int n_tensors, const void* const* g, const int64_t* n, const int* types, int all_types = kPBf16 | kGBf16) {
     ODW_REQUIRE(n_tensors >= 0 && (n_tensors == 0 || (g && n && types)), "%s: null list", what);
     for (int i = 0; i < n_tensors; ++i) {
         ODW_REQUIRE(n[i] >= 0 && n[i] < kMaxElements, "%s: tensor %d has %lld elements", what, i, (long long)n[i]);
         ODW_REQUIRE(n[i] == 0 || g[i], "%s: tensor %d: null pointer", what, i);
-        ODW_REQUIRE(types[i] >= 0 && types[i] <= 3, "%s: tensor %d: bad type %d", what, i, types[i]);
+        ODW_REQUIRE(types[i] >= 0 && types[i] <= all_types, "%s: tensor %d: bad type %d", what, i, types[i]);
         ODW_REQUIRE(aligned(g[i], types[i] & kGBf16 ? 2 : 4), "%s: tensor %d: pointer not aligned to its elements", what, i);
     }
     return ODW_OK;
@@ -484,7 +486,7 @@ int adamw(bool bits8, int n_tensors, void* const* p, const void* const* g, void*
           double eps, int64_t step, const float* bias, const float* grad_scale, float grad_mult, uint32_t k0, uint32_t k1,
           int max_workgroups, hipStream_t stream) {
     const char* what = bits8 ? "adamw8" : "adamw";
-    const int rc = check_list(what, n_tensors, g, n, types);
+    const int rc = check_list(what, n_tensors, g, n, types, kPBf16 | kGBf16 | (bits8 ? kVToZero : 0));
     if (rc != ODW_OK) return rc;
     ODW_REQUIRE(n_tensors == 0 || (p && m && v && lr && wd && (!bits8 || e)), "%s: null list", what);
     ODW_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "%s: betas %g, %g not in [0, 1)", what, beta1, beta2);

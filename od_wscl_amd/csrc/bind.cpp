@@ -181,7 +181,7 @@ void device_scalar(const char* what, const char* name, const Tensor& t, int devi
 void adamw(bool bits8, const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& m, const std::vector<Tensor>& v,
            const std::optional<std::vector<Tensor>>& scales, const py::object& step, const std::vector<int64_t>& key, const py::object& lr,
            const std::vector<double>& betas, double eps, const py::object& weight_decay, const OptTensor& grad_scale,
-           const std::optional<std::vector<OptTensor>>& copies, double grad_mult, int64_t max_workgroups) {
+           const std::optional<std::vector<OptTensor>>& copies, double grad_mult, int64_t max_workgroups, bool hold_v) {
     const char* what = bits8 ? "adamw8_step" : "adamw_step";
     const at::NoGradGuard no_grad;
     if (bits8 && (key.size() != 2 || key[0] < 0 || key[1] < 0 || key[0] >> 32 || key[1] >> 32)) value_error("%s: key has to be two 32-bit integers", what);
@@ -220,7 +220,7 @@ void adamw(bool bits8, const std::vector<Tensor>& params, const std::vector<Tens
     const std::vector<float> lrs = scalars(what, "lr", lr, count), wds = scalars(what, "weight_decay", weight_decay, count);
     if (grad_scale) device_scalar(what, "grad_scale", *grad_scale, device, at::kFloat);
     std::vector<int> types;
-    for (size_t i = 0; i < count; ++i) types.push_back((params[i].scalar_type() == at::kBFloat16 ? 1 : 0) + (grads[i].scalar_type() == at::kBFloat16 ? 2 : 0));
+    for (size_t i = 0; i < count; ++i) types.push_back((params[i].scalar_type() == at::kBFloat16 ? 1 : 0) + (grads[i].scalar_type() == at::kBFloat16 ? 2 : 0) + (bits8 && !hold_v ? 4 : 0));
     const c10::DeviceGuard guard(params[0].device());
     void* stream = stream_of(params[0]);
     Tensor bias;

@@ -8,8 +8,8 @@ that do not train well under SGD.  Three ways in:
   * `adamw_step` / `adamw8_step` / `grad_norm` / `clip_grad_norm_` on lists of tensors.
 
 States are fp32, or 8-bit floats (2 bytes a parameter for both averages instead of 8): the first average in float8_e4m3fn,
-the second in float8_e5m2, a power-of-two scale each for every 256 consecutive elements of a tensor, rounded stochastically with the
-counter-based stream of utils/rng.py -- a step is a function of its inputs and its key, whatever the launch geometry.
+the second in float8_e5m2, a power-of-two scale each for every 256 consecutive elements of a tensor, rounded stochastically with counter-based
+bits (adamw8_step says which) -- a step is a function of its inputs and its key, whatever the launch geometry.
 
 Every tensor is on one GPU; the work goes to the current stream of that device; nothing is read back to the host."""
 import math
@@ -57,18 +57,24 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     GPU (the clip coefficient of grad_norm).  copies: list of bf16 tensors (or None) that get the new params, as the matrix cores read
     them.  max_workgroups: 0, or the width of a pass that runs beside other work."""
     L.bind().adamw(False, params, grads, exp_avgs, exp_avg_sqs, None, step, (), lr, betas, eps, weight_decay, grad_scale, copies, grad_mult,
-                   max_workgroups)
+                   max_workgroups, True)
 
 
 def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, scales, step, key, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
-                grad_scale=None, copies=None, grad_mult=1.0, max_workgroups=0):
+                grad_scale=None, copies=None, grad_mult=1.0, max_workgroups=0, hold_v=True):
     """adamw_step with 8-bit states: exp_avgs float8_e4m3fn, exp_avg_sqs float8_e5m2, scales uint8 (ceil(n / 256), 2): exponent + 127 of
     the power-of-two scales of the two averages of 256 elements; value = code * 2^(scale - 127) (state8_zeros, state8_read,
-    state8_write); a second average that is not zero is held as 2^-16 of its scale at least.  The update uses the averages before they are rounded.  key: two 32-bit integers, other ones every step
-    (utils.rng.stream_key(seed, step)); the random bits of an element depend on the key and on its position in the concatenation of
-    `params`.  With `step` on the GPU the step's number is added to key[1].  An average that is not finite is held as NaN."""
+    state8_write).  The update uses the averages before they are rounded.  An average that is not finite is held as NaN.
+
+    key: two 32-bit integers, other ones every step (utils.rng.stream_key(seed, step)).  The random bits of an element are mix(mix(i ^ k0)
+    + k1) of utils/rng.py, i = its position in the concatenation of `params`, under the keys k0 = key[0] and k1 = key[1] + 0x9E3779B9 key[0]:
+    keys that differ in the first word alone (a step's number, say) then do not permute one set of numbers over the elements.  With
+    `step` on the GPU the step's number is added to k1.
+
+    hold_v: a second average that is not zero is held as 2^-16 of its scale at least, which bounds the steps of elements far below their block's
+    largest.  False: it is rounded to zero like any other value, and such an element may move by lr times its first average over eps."""
     L.bind().adamw(True, params, grads, exp_avgs, exp_avg_sqs, scales, step, key, lr, betas, eps, weight_decay, grad_scale, copies, grad_mult,
-                   max_workgroups)
+                   max_workgroups, hold_v)
 
 
 # ---- the 8-bit states as tensors -----------------------------------------------------------------------------------------------------
