@@ -372,7 +372,8 @@ def run_own(s):
     if case["op"] == "adamw":
         optim.adamw_step(s["p"], s["g"], s["m"], s["v"], s["step"], **more)
     else:
-        optim.adamw8_step(s["p"], s["g"], s["m"], s["v"], s["e"], s["step"], key_of(s["seed"], s["step"]), **more)
+        k0, k1 = key_of(s["seed"], s["step"])         # the stream's words; adamw8_step adds 0x9E3779B9 key[0] to the second one
+        optim.adamw8_step(s["p"], s["g"], s["m"], s["v"], s["e"], s["step"], (k0, (k1 - 0x9E3779B9 * k0) & 0xFFFFFFFF), hold_v=False, **more)
     return step_outputs(s)
 
 
