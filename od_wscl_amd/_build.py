@@ -4,6 +4,7 @@ hipcc cross-compiles without a GPU, so this also runs in the CPU-only build
 container; the resulting .so is git-ignored but ships with gpurun snapshots.
 """
 import glob
+import json
 import os
 import subprocess
 
@@ -11,6 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libodwscl.so")
 BIND, BIND_SRC = os.path.join(HERE, "_bind.so"), os.path.join(CSRC, "bind.cpp")
+RECORD = os.path.join(HERE, "build", "commands.json")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 # -ffp-contract=off: ROI bin / sample coordinates must round exactly like the
@@ -43,8 +45,40 @@ def _bind_command():
              "-ltorch", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN"])
 
 
+def _object(src):
+    return os.path.splitext(src)[0] + ".o"
+
+
+def _commands():
+    """Every output and the command that makes it: an output whose command was another one (other flags, a source that came or went, another
+    torch) is as stale as one that is older than its sources."""
+    import torch
+    cmds = {_object(src): [HIPCC] + FLAGS + ["-c", src, "-o", _object(src)] for src in sources()}
+    cmds[LIB] = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", LIB] + [_object(src) for src in sources()]
+    cmds[BIND] = _bind_command()
+    return cmds, {out: [a.replace(HERE, ".") for a in cmd] + ([torch.__version__] if out == BIND else []) for out, cmd in cmds.items()}
+
+
+def _recorded():
+    try:
+        with open(RECORD) as f:
+            return json.load(f)
+    except (OSError, ValueError):
+        return {}
+
+
+def _record(made):
+    os.makedirs(os.path.dirname(RECORD), exist_ok=True)
+    with open(RECORD + ".new", "w") as f:
+        json.dump(made, f, indent=1, sort_keys=True)
+    os.replace(RECORD + ".new", RECORD)
+
+
 def _stale():
     if not os.path.exists(LIB) or not os.path.exists(BIND):
+        return True
+    made = _recorded()
+    if any(made.get(os.path.basename(out)) != how for out, how in _commands()[1].items()):
         return True
     t = min(os.path.getmtime(LIB), os.path.getmtime(BIND))
     deps = sources() + [BIND_SRC] + glob.glob(os.path.join(CSRC, "*.h")) + \
@@ -56,16 +90,20 @@ def build(force=False, verbose=False):
     """Compile csrc/*.hip -> libodwscl.so (objects cached next to the sources), csrc/bind.cpp -> _bind.so."""
     if not force and not _stale():
         return LIB
-    objs = []
+    cmds, how = _commands()
+    name = os.path.basename
+    made = {} if force else {name(out): how[out] for out in cmds if out != LIB and _recorded().get(name(out)) == how[out]}
+    _record(made)                       # (what is about to be made again is not recorded until it is there)
     procs = []
     for src in sources():
-        obj = os.path.splitext(src)[0] + ".o"
-        objs.append(obj)
+        obj = _object(src)
         newest_dep = max([os.path.getmtime(src)] + [os.path.getmtime(h) for h in
                          glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(HERE, "..", "include", "*.h"))])
-        if not force and os.path.exists(obj) and os.path.getmtime(obj) > newest_dep:
+        if name(obj) in made and os.path.exists(obj) and os.path.getmtime(obj) > newest_dep:
             continue
-        cmd = [HIPCC] + FLAGS + ["-c", src, "-o", obj]
+        cmd = cmds[obj]
+        made.pop(name(obj), None)
+        _record(made)
         if verbose:
             print(" ".join(cmd))
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
@@ -75,14 +113,17 @@ def build(force=False, verbose=False):
             raise RuntimeError("hipcc failed on %s:\n%s" % (src, out.decode()))
         if verbose and out:
             print(out.decode())
-    cmd = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", LIB] + objs
-    subprocess.check_call(cmd)
+        made[name(_object(src))] = how[_object(src)]
+    subprocess.check_call(cmds[LIB])
+    made[name(LIB)] = how[LIB]
+    _record(made)
     newest = max(os.path.getmtime(p) for p in [BIND_SRC] + glob.glob(os.path.join(HERE, "..", "include", "*.h")))
-    if force or not os.path.exists(BIND) or os.path.getmtime(BIND) <= newest:
-        cmd = _bind_command()
+    if name(BIND) not in made or not os.path.exists(BIND) or os.path.getmtime(BIND) <= newest:
         if verbose:
-            print(" ".join(cmd))
-        subprocess.check_call(cmd)
+            print(" ".join(cmds[BIND]))
+        subprocess.check_call(cmds[BIND])
+        made[name(BIND)] = how[BIND]
+        _record(made)
     else:
         os.utime(BIND)
     return LIB
