@@ -47,6 +47,8 @@ std::string format(const char* fmt, va_list ap) {
 }
 void need_gpu(const Tensor& t) {
     if (!t.is_cuda()) throw std::runtime_error("od_wscl_amd: tensor is not on the GPU -- the hot path has no CPU implementation");
+    // (the stand-ins of torch.func's transforms)
+    if (t.layout() == at::kStrided && !t.has_storage()) throw std::runtime_error("od_wscl_amd: tensor has no memory of its own -- a transform's stand-in");
 }
 void check(int code, const char* what) {
     if (code != 0) throw std::runtime_error(std::string(what) + " failed (" + std::to_string(code) + "): " + odw_last_error());
@@ -361,6 +363,9 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
 
 py::object rms_norm(const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps) {
     check_rows("rms_norm", x, weight, residual, eps);
+    // (outputs without a tangent would be taken for constant; no_grad does not end forward mode)
+    for (const Tensor* t : {&x, weight ? &*weight : nullptr, residual ? &*residual : nullptr})
+        if (t && t->_fw_grad(0).defined()) throw std::runtime_error("rms_norm: has no forward-mode derivative");
     if (at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (residual && residual->requires_grad()))) {
         const auto out = RMSNorm::apply(x, weight, residual, eps);
         return residual ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);

@@ -33,7 +33,7 @@ def grad_norm(grads, max_norm=None):
     """The 2-norm over all of `grads` (tensors, or parameters that stand for their .grad; or one) as a 0-dim fp32 tensor; summed in fp64 in
     one order, so the same from run to run.  With max_norm: (norm, coef), coef = min(1, max_norm / (norm + 1e-6)) -- the factor
     that clips them, for `grad_scale` of adamw_step (clipping without a pass over the gradients).  Neither is read by the host.
-    A non-finite gradient makes the norm inf or NaN, and coef 0 or NaN."""
+    A non-finite gradient makes the norm inf or NaN, and coef 0 or NaN.  Not differentiable."""
     return L.bind().grad_norm(_list(grads), max_norm)
 
 

@@ -1,0 +1,32 @@
+"""Derivatives that layers.rms_norm does not have are refused, not taken for zero."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "residual"])
+def test_forward_mode(which):
+    from od_wscl_amd import layers
+    x, w, r = (torch.randn(*s, device="cuda") for s in ((4, 32), (32,), (4, 32)))
+    with fw.dual_level():
+        args = dict(x=x, weight=w, residual=r)
+        layers.rms_norm(**args)                                 # nothing carries a tangent: as ever
+        args[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            layers.rms_norm(**args)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            layers.rms_norm(**args)
+        args = {k: v.detach().requires_grad_(True) if k != which else v for k, v in args.items()}
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            layers.rms_norm(**args)
+
+
+def test_function_transforms():
+    from od_wscl_amd import layers
+    x = torch.randn(4, 32, device="cuda")
+    for call in (lambda: torch.func.jvp(layers.rms_norm, (x,), (x,)), lambda: torch.func.vmap(layers.rms_norm)(x[None]),
+                 lambda: torch.func.grad(lambda a: layers.rms_norm(a).sum())(x)):
+        with pytest.raises(RuntimeError):
+            call()
