@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -52,6 +53,10 @@ void need_gpu(const Tensor& t) {
 }
 void check(int code, const char* what) {
     if (code != 0) throw std::runtime_error(std::string(what) + " failed (" + std::to_string(code) + "): " + odw_last_error());
+}
+// (a trace would record the empty outputs and not the launches that fill them)
+void not_traced(const char* what) {
+    if (torch::jit::tracer::isTracing()) throw std::runtime_error(std::string(what) + ": cannot be traced");
 }
 std::string name_of(at::ScalarType t) { return std::string("torch.") + at::toString(t); }
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
@@ -112,6 +117,7 @@ const Types kFloats = {at::kFloat, at::kBFloat16};
 
 // out[0] = the norm, out[1] = the factor that clips it.
 Tensor norm_of(const char* what, const std::vector<Tensor>& grads, double max_norm, bool written) {
+    not_traced(what);
     if (grads.empty()) value_error("%s: no gradients", what);
     need_gpu(grads[0]);
     const std::vector<int64_t> n = sizes_of(grads);
@@ -185,6 +191,7 @@ void adamw(bool bits8, const std::vector<Tensor>& params, const std::vector<Tens
            const std::vector<double>& betas, double eps, const py::object& weight_decay, const OptTensor& grad_scale,
            const std::optional<std::vector<OptTensor>>& copies, double grad_mult, int64_t max_workgroups, bool hold_v) {
     const char* what = bits8 ? "adamw8_step" : "adamw_step";
+    not_traced(what);
     const at::NoGradGuard no_grad;
     if (bits8 && (key.size() != 2 || key[0] < 0 || key[1] < 0 || key[0] >> 32 || key[1] >> 32)) value_error("%s: key has to be two 32-bit integers", what);
     if (params.empty()) return;
@@ -269,6 +276,7 @@ bool is_bf16(at::ScalarType t) { return t == at::kBFloat16; }
 void* ptr(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 
 void check_rows(const char* what, const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps) {
+    not_traced(what);
     need_gpu(x);
     if (x.dim() < 1 || x.size(-1) < 1) value_error("%s: x has no columns", what);
     if (x.size(-1) > INT32_MAX) value_error("%s: x has %lld columns", what, (long long)x.size(-1));

@@ -1,4 +1,4 @@
-"""Derivatives that layers.rms_norm does not have are refused, not taken for zero."""
+"""Derivatives that layers.rms_norm does not have are refused, not taken for zero; so are traces, which would not hold the launches."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
@@ -30,3 +30,15 @@ def test_function_transforms():
                  lambda: torch.func.grad(lambda a: layers.rms_norm(a).sum())(x)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_traces():
+    from od_wscl_amd import layers, optim
+    x = torch.randn(4, 32, device="cuda")
+
+    def step(a):
+        optim.adamw_step([a], [a.clone()], [torch.zeros_like(a)], [torch.zeros_like(a)], 1)
+        return a
+    for f in (layers.RMSNorm(32).cuda(), lambda a: layers.rms_norm_fp8(a)[1], step, lambda a: optim.grad_norm([a]), lambda a: optim.clip_grad_norm_([a], 1.0)):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, (x.clone(),), check_trace=False)
