@@ -287,18 +287,27 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1) void rms_
     // (the values again, from where they came: their registers hold the products)
     auto value = [&](int i) { return res ? up(h[r * D + i]) : up(x[r * ldx + i]); };
     auto gain = [&](int i) { return w ? ld(w, types & kWBf16, i) : 1.0f; };
-    // e of the largest product (of equal ones the largest e; of equal ones in one thread the last one's), as a word that grows with it
+    // e of the largest product (of equal ones, in this thread and over the threads, the largest e), as a word that grows with it.  The thread
+    // that holds it loads its elements again: looked for in v they would stay in registers until here, and the widest forms spill (2000 x
+    // 25088 fp32 69-71 us for 64)
     uint32_t key = 0;
     if (best == __float_as_uint(pm)) {
-        int at = 0;
+#pragma clang loop unroll_count(2)
+        for (int k = 0; k < VPT; ++k) {
+            const int i = (k * TPR + t) * V;
+            if (i >= D) break;
+            float hv[V], gv[V];
+            if (res) load<TH, V>(h + r * D + i, D - i, hv);
+            else load<TX, V>(x + r * ldx + i, D - i, hv);
+            load_w<V>(w, types & kWBf16, i, D - i, gv);
 #pragma unroll
-        for (int k = 0; k < VPT; ++k)
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if ((__float_as_uint(v[k][j]) & 0x7FFFFFFFu) == best) at = (k * TPR + t) * V + j;
-        const float hv = value(at), gv = gain(at), p = hv * gv;
-        const uint32_t e = __float_as_uint(p < 0.0f ? -fmaf(hv, gv, -p) : fmaf(hv, gv, -p));
-        key = (e >> 31) ? ~e : e | 0x80000000u;
+            for (int j = 0; j < V; ++j) {
+                const float p = hv[j] * gv[j];
+                const uint32_t e = __float_as_uint(p < 0.0f ? -fmaf(hv[j], gv[j], -p) : fmaf(hv[j], gv[j], -p));
+                const uint32_t word = (e >> 31) ? ~e : e | 0x80000000u;
+                if ((__float_as_uint(p) & 0x7FFFFFFFu) == best) key = key > word ? key : word;
+            }
+        }
     }
     key = row_max<TPR>(key, part[0]);
     const double tmax = (double)pm + (double)__uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
