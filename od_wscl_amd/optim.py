@@ -130,7 +130,8 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits: 32, or 8.  max_grad_norm: clip the gradients' common 2-norm (over all groups) within the step.  seed: of the 8-bit
     states' rounding.  capturable: the step's number lives on the GPU, so that step() can be captured into a HIP graph (learning
-    rates are then those of the capture).
+    rates are then those of the capture).  A captured step's parameters keep their step numbers together: an eager step of other betas or
+    with a gradient missing gives some of them numbers of their own, and the step has to be captured again.
 
     state_dict() holds the averages in fp32 whatever state_bits is (an 8-bit state is read exactly and comes back the same), so
     checkpoints move between 32 and 8 bits and torch.optim.AdamW."""
@@ -187,7 +188,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        calls, grads, fresh = {}, [], {}
+        calls, grads, fresh = {}, [], {}          # (fresh: the counters made in this step)
         for group in self.param_groups:
             for p in group["params"]:
                 if p.grad is None:
@@ -195,19 +196,20 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad.is_sparse:
                     raise TypeError("AdamW: sparse gradient")
                 st = self._state(p)
+                rule = (tuple(group["betas"]), group["eps"])
                 if st["step"] is None:
-                    st["step"] = fresh.setdefault(p.device, torch.zeros(1, dtype=torch.int64, device=p.device)) if self.capturable else 0
+                    st["step"] = self._counter(fresh, (p.device,) + rule, 0, p.device) if self.capturable else 0
                 g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
                 grads.append(g)
                 number = id(st["step"]) if self.capturable else st["step"]
-                calls.setdefault((tuple(group["betas"]), group["eps"], number), []).append((group, p, g, st))
+                calls.setdefault(rule + (number,), []).append((group, p, g, st))
         if not grads:
             return loss
         coef = None
         if self.max_grad_norm is not None:
             self.grad_norm, coef = grad_norm(grads, self.max_grad_norm)
         if self.capturable:
-            self._check_shared_steps(calls)
+            self._part_counters(calls)
         for ci, ((betas, eps, _), items) in enumerate(calls.items()):
             step = items[0][3]["step"]
             if not self.capturable:
@@ -226,16 +228,33 @@ class AdamW(torch.optim.Optimizer):
                     x[3]["step"] = step
         return loss
 
-    def _check_shared_steps(self, calls):
-        """Parameters that took their first step together share one counter on the GPU: it is advanced once, for all of them."""
-        have = [(x[3]["step"], x[1]) for items in calls.values() for x in items]
-        if len(set(id(s) for s, _ in have)) != len(calls):
-            raise RuntimeError("AdamW: capturable parameters that share a step counter have other betas or eps")
-        stepped = set(id(p) for _, p in have)
-        counters = set(id(s) for s, _ in have)
+    @staticmethod
+    def _counter(made, key, value, device):
+        if key not in made:
+            made[key] = torch.full((1,), value, dtype=torch.int64, device=device)
+        return made[key]
+
+    def _part_counters(self, calls):
+        """Parameters that took their first step together, by one rule, share a counter on the GPU: a step advances it once, for all of them.
+        Those that part -- by a group's new betas or eps, or because only some have a gradient -- get counters of their own here; a step that
+        is being captured cannot do that (its replays would take the copies' values anew)."""
+        stepped = set(id(x[1]) for items in calls.values() for x in items)
+        taken, apart = set(), {}
+        for items in calls.values():
+            counter = items[0][3]["step"]
+            if id(counter) in taken:             # (another rule's call has it)
+                apart[id(items[0][1])] = counter, [x[3] for x in items]
+            taken.add(id(counter))
         for p, st in self.state.items():
-            if id(st.get("step")) in counters and id(p) not in stepped:
-                raise RuntimeError("AdamW: a parameter without a gradient shares the step counter of others that have one (capturable)")
+            if id(st.get("step")) in taken and id(p) not in stepped:
+                apart.setdefault(("rest", id(st["step"])), (st["step"], []))[1].append(st)
+        if apart and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: parameters that share a step counter part in a captured step (other betas or eps, or a missing gradient): take "
+                               "such a step before the capture")
+        for counter, states in apart.values():
+            own = counter.clone()
+            for st in states:
+                st["step"] = own
 
     def state_dict(self):
         """torch.optim.AdamW's layout: {"step": fp32 tensor, "exp_avg", "exp_avg_sq": fp32} a parameter."""
@@ -256,6 +275,7 @@ class AdamW(torch.optim.Optimizer):
         shared = {}
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         own = [p for g in self.param_groups for p in g["params"]]
+        rules = {id(p): (tuple(g["betas"]), g["eps"]) for g in self.param_groups for p in g["params"]}
         for i, p in zip(saved, own):
             if i not in states:
                 continue
@@ -268,4 +288,5 @@ class AdamW(torch.optim.Optimizer):
                 st["exp_avg"], st["exp_avg_sq"] = m.clone(), v.clone()
             st["step"] = step
             if self.capturable:
-                st["step"] = shared.setdefault((p.device, step), torch.full((1,), step, dtype=torch.int64, device=p.device))
+                rule = rules[id(p)]
+                st["step"] = self._counter(shared, (p.device, step) + rule, step, p.device)
