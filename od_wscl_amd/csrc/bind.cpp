@@ -226,6 +226,8 @@ void adamw(bool bits8, const std::vector<Tensor>& params, const std::vector<Tens
     // (a gradient whose square is nothing in fp32, below 1e-21, then moves p by at most lr * 1e-6, not by lr * g / eps of any size)
     if (!(eps >= 1e-15 && std::isfinite((float)eps))) value_error("%s: eps = %g", what, eps);
     if (!std::isfinite((float)grad_mult)) value_error("%s: grad_mult = %g", what, grad_mult);
+    // (all refusals come before the step's number on the GPU moves)
+    if (max_workgroups < 0) throw std::runtime_error(std::string(what) + ": max_workgroups = " + std::to_string(max_workgroups));
     const std::vector<float> lrs = scalars(what, "lr", lr, count), wds = scalars(what, "weight_decay", weight_decay, count);
     if (grad_scale) device_scalar(what, "grad_scale", *grad_scale, device, at::kFloat);
     std::vector<int> types;
@@ -251,7 +253,7 @@ void adamw(bool bits8, const std::vector<Tensor>& params, const std::vector<Tens
     const float* bp = bias.defined() ? bias.data_ptr<float>() : nullptr;
     const float* gs = grad_scale ? grad_scale->data_ptr<float>() : nullptr;
     void* const* cp = ac.empty() ? nullptr : ac.data();
-    const int wide = (int)std::min<int64_t>(std::max<int64_t>(max_workgroups, -1), INT32_MAX);
+    const int wide = (int)std::min<int64_t>(max_workgroups, INT32_MAX);
     if (bits8)
         check(odw_adamw8((int)count, ap.data(), ag.data(), am.data(), av.data(), (uint8_t* const*)ae.data(), cp, n.data(), types.data(), lrs.data(),
                          wds.data(), betas[0], betas[1], eps, number, bp, gs, (float)grad_mult, (uint32_t)key[0], (uint32_t)key[1], wide, stream), what);

@@ -99,3 +99,17 @@ def test_one_fill_for_many_parameters():
         p.grad = torch.ones_like(p)
     o.step()
     assert len(set(id(o.state[p]["step"]) for p in ps)) == 1
+
+
+@pytest.mark.parametrize("bad", [dict(max_workgroups=-1), dict(lr=-1.0), dict(eps=0.0), dict(betas=(1.0, 0.9)), dict(grad_mult=float("nan")),
+                                 dict(copies=[]), dict(exp_avgs=[torch.zeros(7)]), dict(grad_scale=torch.ones(2))], ids=lambda d: list(d)[0])
+def test_a_refused_step_leaves_its_number(bad):
+    from od_wscl_amd import optim
+    one = lambda: [torch.ones(8, device="cuda")]           # noqa: E731
+    step = torch.full((1,), 4, dtype=torch.int64, device="cuda")
+    args = dict(params=one(), grads=one(), exp_avgs=one(), exp_avg_sqs=one(), step=step)
+    with pytest.raises((ValueError, RuntimeError)):
+        optim.adamw_step(**{**args, **bad})
+    assert int(step) == 4 and torch.equal(args["params"][0], one()[0])
+    optim.adamw_step(**args)
+    assert int(step) == 5
