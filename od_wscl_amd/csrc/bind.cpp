@@ -78,9 +78,9 @@ std::string names_of(const Types& types) {
 }
 
 // `list` beside the first one: as many, on its GPU, contiguous, of one of `types` and of `sizes`; their addresses.  What is written must not be in
-// a list twice (two workgroups would update it at once).
+// a list twice (two workgroups would update it at once).  Where signs matter a lazily negated view, whose memory holds the other ones, is refused.
 std::vector<void*> addresses(const char* what, const char* name, const std::vector<Tensor>& list, int device, const std::vector<int64_t>& sizes,
-                             const Types& types, bool written) {
+                             const Types& types, bool written, bool signs = true) {
     if (list.size() != sizes.size()) value_error("%s: %zu %s for %zu tensors", what, list.size(), name, sizes.size());
     std::vector<void*> at;
     at.reserve(list.size());
@@ -95,6 +95,7 @@ std::vector<void*> addresses(const char* what, const char* name, const std::vect
                        names_of(types).c_str());
         if (t.numel() != sizes[i]) value_error("%s: %s[%zu] has %lld elements, %lld wanted", what, name, i, (long long)t.numel(), (long long)sizes[i]);
         if (!t.is_contiguous()) value_error("%s: %s[%zu] is not contiguous", what, name, i);
+        if (signs && t.is_neg()) value_error("%s: %s[%zu] is a negated view (resolve_neg)", what, name, i);
         at.push_back(t.numel() ? t.data_ptr() : nullptr);
     }
     if (written) {
@@ -121,7 +122,7 @@ Tensor norm_of(const char* what, const std::vector<Tensor>& grads, double max_no
     if (grads.empty()) value_error("%s: no gradients", what);
     need_gpu(grads[0]);
     const std::vector<int64_t> n = sizes_of(grads);
-    const std::vector<void*> at = addresses(what, "grads", grads, grads[0].get_device(), n, kFloats, written);
+    const std::vector<void*> at = addresses(what, "grads", grads, grads[0].get_device(), n, kFloats, written, false);
     if (!(max_norm > 0.0)) value_error("%s: max_norm = %g", what, max_norm);
     std::vector<int> types;
     for (const Tensor& g : grads) types.push_back(g.scalar_type() == at::kBFloat16 ? 2 : 0);
@@ -269,9 +270,9 @@ void adamw(bool bits8, const std::vector<Tensor>& params, const std::vector<Tens
 
 // ---- the norm of rows ---------------------------------------------------------------------------------------------------------------
 
-// (rows, D) view with dense columns; a copy only where there is none.
-Tensor rows(const Tensor& t, int64_t D) {
-    Tensor r = t.dim() == 2 ? t : t.reshape({-1, D});
+// (rows, D) view with dense columns; a copy only where there is none (or its negation is not in memory yet).
+Tensor rows(const Tensor& any, int64_t D) {
+    const Tensor t = any.resolve_neg(), r = t.dim() == 2 ? t : t.reshape({-1, D});
     return r.stride(1) == 1 || D == 1 ? r : r.contiguous();
 }
 bool is_bf16(at::ScalarType t) { return t == at::kBFloat16; }
@@ -303,7 +304,7 @@ int types_of(at::ScalarType x, at::ScalarType h, const Tensor& w) { return is_bf
 // The forward launch into `out` (y, or with `scale` the 8-bit codes); h is undefined without a residual.
 Tensor norm_rows(const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps, const Tensor& out, const Tensor& rstd, const Tensor& scale) {
     const int64_t D = x.size(-1);
-    const Tensor x2 = rows(x, D), r2 = residual ? rows(*residual, D) : Tensor(), w = weight ? weight->contiguous() : Tensor();
+    const Tensor x2 = rows(x, D), r2 = residual ? rows(*residual, D) : Tensor(), w = weight ? weight->resolve_neg().contiguous() : Tensor();
     const Tensor h = residual ? at::empty(x.sizes(), residual->options()) : Tensor();
     const int types = types_of(x.scalar_type(), (residual ? *residual : x).scalar_type(), w);
     const int64_t R = x2.size(0), ldx = x2.stride(0), ldr = residual ? r2.stride(0) : 0;
@@ -357,7 +358,7 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
         }
         const c10::DeviceGuard guard(h.device());
         const int64_t D = h.size(-1);
-        const Tensor h2 = rows(h, D), g2 = rows(dy, D), d2 = dh.defined() ? rows(dh, D) : Tensor(), w = weight.defined() ? weight.contiguous() : Tensor();
+        const Tensor h2 = rows(h, D), g2 = rows(dy, D), d2 = dh.defined() ? rows(dh, D) : Tensor(), w = weight.defined() ? weight.resolve_neg().contiguous() : Tensor();
         const int64_t R = h2.size(0);
         const bool mixed = h_type != x_type;
         const Tensor dx = need_x || (need_r && !mixed) ? at::empty(h.sizes(), h.options().dtype(x_type)) : Tensor();

@@ -199,7 +199,7 @@ class AdamW(torch.optim.Optimizer):
                 rule = (tuple(group["betas"]), group["eps"])
                 if st["step"] is None:
                     st["step"] = self._counter(fresh, (p.device,) + rule, 0, p.device) if self.capturable else 0
-                g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
+                g = p.grad.resolve_neg().contiguous()
                 grads.append(g)
                 number = id(st["step"]) if self.capturable else st["step"]
                 calls.setdefault(rule + (number,), []).append((group, p, g, st))
