@@ -161,7 +161,9 @@ py::object grad_norm(const std::vector<Tensor>& items, std::optional<double> max
 
 Tensor clip_grad_norm(const std::vector<Tensor>& items, double max_norm) {
     const at::NoGradGuard no_grad;
-    return norm_of("clip_grad_norm_", grads_of("clip_grad_norm_", items, false), max_norm, true).select(0, 0);
+    const std::vector<Tensor> grads = grads_of("clip_grad_norm_", items, false);
+    if (grads.empty() && max_norm > 0.0) return at::zeros({}, (items.empty() ? at::TensorOptions() : items[0].options()).dtype(at::kFloat));
+    return norm_of("clip_grad_norm_", grads, max_norm, true).select(0, 0);
 }
 
 std::vector<float> scalars(const char* what, const char* name, const py::object& value, size_t n) {
