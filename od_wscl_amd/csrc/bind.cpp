@@ -78,9 +78,10 @@ std::string names_of(const Types& types) {
 }
 
 // `list` beside the first one: as many, on its GPU, contiguous, of one of `types` and of `sizes`; their addresses.  What is written must not be in
-// a list twice (two workgroups would update it at once).  Where signs matter a lazily negated view, whose memory holds the other ones, is refused.
+// a list twice (two workgroups would update it at once).  `alone` (a norm, a scaling): elements go with no other list's, so that any order without
+// gaps will do, and a lazily negated view too, whose memory holds the other sign.
 std::vector<void*> addresses(const char* what, const char* name, const std::vector<Tensor>& list, int device, const std::vector<int64_t>& sizes,
-                             const Types& types, bool written, bool signs = true) {
+                             const Types& types, bool written, bool alone = false) {
     if (list.size() != sizes.size()) value_error("%s: %zu %s for %zu tensors", what, list.size(), name, sizes.size());
     std::vector<void*> at;
     at.reserve(list.size());
@@ -94,8 +95,8 @@ std::vector<void*> addresses(const char* what, const char* name, const std::vect
             type_error("%s: %s[%zu] is %s%s (%s)", what, name, i, t.layout() != at::kStrided ? "sparse " : "", name_of(t.scalar_type()).c_str(),
                        names_of(types).c_str());
         if (t.numel() != sizes[i]) value_error("%s: %s[%zu] has %lld elements, %lld wanted", what, name, i, (long long)t.numel(), (long long)sizes[i]);
-        if (!t.is_contiguous()) value_error("%s: %s[%zu] is not contiguous", what, name, i);
-        if (signs && t.is_neg()) value_error("%s: %s[%zu] is a negated view (resolve_neg)", what, name, i);
+        if (alone ? !t.is_non_overlapping_and_dense() : !t.is_contiguous()) value_error("%s: %s[%zu] is not contiguous", what, name, i);
+        if (!alone && t.is_neg()) value_error("%s: %s[%zu] is a negated view (resolve_neg)", what, name, i);
         at.push_back(t.numel() ? t.data_ptr() : nullptr);
     }
     if (written) {
@@ -122,7 +123,7 @@ Tensor norm_of(const char* what, const std::vector<Tensor>& grads, double max_no
     if (grads.empty()) value_error("%s: no gradients", what);
     need_gpu(grads[0]);
     const std::vector<int64_t> n = sizes_of(grads);
-    const std::vector<void*> at = addresses(what, "grads", grads, grads[0].get_device(), n, kFloats, written, false);
+    const std::vector<void*> at = addresses(what, "grads", grads, grads[0].get_device(), n, kFloats, written, true);
     if (!(max_norm > 0.0)) value_error("%s: max_norm = %g", what, max_norm);
     std::vector<int> types;
     for (const Tensor& g : grads) types.push_back(g.scalar_type() == at::kBFloat16 ? 2 : 0);
@@ -147,7 +148,7 @@ std::vector<Tensor> grads_of(const char* what, const std::vector<Tensor>& items,
         const Tensor g = t.requires_grad() && t.is_leaf() ? t.grad() : t.detach();
         if (!g.defined()) continue;
         if (g.layout() != at::kStrided) type_error("%s: gradient %zu is sparse", what, grads.size());
-        grads.push_back(any_layout ? g.contiguous() : g);
+        grads.push_back(any_layout && !g.is_non_overlapping_and_dense() ? g.contiguous() : g);
     }
     return grads;
 }

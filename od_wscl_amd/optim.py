@@ -39,7 +39,7 @@ def grad_norm(grads, max_norm=None):
 
 def clip_grad_norm_(grads, max_norm):
     """Scale all of `grads` (tensors, or parameters that stand for their .grad; or one) in place so that their common 2-norm is at most
-    max_norm; returns the norm before that, 0 where none has a gradient (torch.nn.utils.clip_grad_norm_, without a host read)."""
+    max_norm (their elements in any order without gaps); returns the norm before that, 0 where none has a gradient (torch.nn.utils.clip_grad_norm_, without a host read)."""
     return L.bind().clip_grad_norm(_list(grads), max_norm)
 
 
