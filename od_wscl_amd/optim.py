@@ -125,8 +125,27 @@ def refuse_other_rules(param_groups):
             raise ValueError("AdamW: the state is of an optimiser with %s" % ", ".join(other))
 
 
+def _order(p):
+    """The order of p's dimensions in memory where that is another one without gaps, else None."""
+    if p.is_contiguous():
+        return None
+    order = sorted(range(p.dim()), key=lambda d: -p.stride(d))
+    return order if p.permute(order).is_contiguous() else None
+
+
+def _flat(t, order):
+    """t's dimensions in that order: contiguous, if t lies like the parameter it is of."""
+    return t if order is None else t.permute(order)
+
+
+def _back(t, order):
+    """What _flat undoes."""
+    return t if order is None else t.permute([order.index(d) for d in range(len(order))])
+
+
 class AdamW(torch.optim.Optimizer):
-    """torch.optim.AdamW's arguments, groups and state names on the kernels above.
+    """torch.optim.AdamW's arguments, groups and state names on the kernels above.  Parameters' elements may lie in any order without gaps
+    (channels_last weights); the averages lie like them.
 
     state_bits: 32, or 8.  max_grad_norm: clip the gradients' common 2-norm (over all groups) within the step.  seed: of the 8-bit
     states' rounding.  capturable: the step's number lives on the GPU, so that step() can be captured into a HIP graph (learning
@@ -167,20 +186,41 @@ class AdamW(torch.optim.Optimizer):
             for st in self.state.values():
                 st.update({k: st[k].view(t) for k, t in STATE8.items()})
 
-    def _state(self, p):
+    def _state(self, p, order):
         st = self.state[p]
         if not st:
             if p.is_cuda and torch.cuda.is_current_stream_capturing():
                 del self.state[p]
                 raise RuntimeError("AdamW: a parameter's first step is being captured: every replay would start it from zero averages again "
                                    "(take a step, or load a state, before the capture)")
-            if self.state_bits == 8:
-                st["exp_avg"], st["exp_avg_sq"], st["scales"] = state8_zeros(p)
-            else:
-                st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
-                st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+            self._hold(st, p, order)
             st["step"] = None            # (set by step(): a number, or with `capturable` a tensor that parameters share)
+        elif not _flat(st["exp_avg"], order).is_contiguous():               # (the parameter was laid out anew)
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: a parameter's elements lie in another order than in the last step; take a step before the capture")
+            self._hold(st, p, order, *self._averages(st))
         return st
+
+    def _hold(self, st, p, order, m=None, v=None):
+        """The averages m and v (fp32; none: zeros) in p's order, as they are held."""
+        flat = _flat(p, order)
+        if self.state_bits == 8:
+            state = state8_zeros(flat) if m is None else state8_write(*(_flat(x, order).contiguous() for x in (m, v)))
+            st["scales"] = state[2]
+        else:
+            state = [torch.zeros_like(flat, dtype=torch.float32, memory_format=torch.contiguous_format) for _ in range(2)]
+            for x, given in zip(state, (m, v)):
+                if given is not None:
+                    x.copy_(_flat(given, order))
+        st["exp_avg"], st["exp_avg_sq"] = (_back(x, order) for x in state[:2])
+
+    @staticmethod
+    def _averages(st):
+        """Both averages in fp32: of an 8-bit state what it holds."""
+        if "scales" not in st:
+            return st["exp_avg"], st["exp_avg_sq"]
+        order = _order(st["exp_avg"])
+        return tuple(_back(x, order) for x in state8_read(*(_flat(st[k], order) for k in STATE8), st["scales"]))
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -195,14 +235,15 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if p.grad.is_sparse:
                     raise TypeError("AdamW: sparse gradient")
-                st = self._state(p)
+                order = _order(p)
+                st = self._state(p, order)
                 rule = (tuple(group["betas"]), group["eps"])
                 if st["step"] is None:
                     st["step"] = self._counter(fresh, (p.device,) + rule, 0, p.device) if self.capturable else 0
-                g = p.grad.resolve_neg().contiguous()
+                g = _flat(p.grad.resolve_neg(), order).contiguous()
                 grads.append(g)
                 number = id(st["step"]) if self.capturable else st["step"]
-                calls.setdefault(rule + (number,), []).append((group, p, g, st))
+                calls.setdefault(rule + (number,), []).append((group, p, g, st, order))
         if not grads:
             return loss
         coef = None
@@ -214,8 +255,8 @@ class AdamW(torch.optim.Optimizer):
             step = items[0][3]["step"]
             if not self.capturable:
                 step += 1
-            ps, gs = [x[1] for x in items], [x[2] for x in items]
-            m, v = ([x[3][k] for x in items] for k in ("exp_avg", "exp_avg_sq"))
+            ps, gs = [_flat(x[1], x[4]) for x in items], [x[2] for x in items]
+            m, v = ([_flat(x[3][k], x[4]) for x in items] for k in ("exp_avg", "exp_avg_sq"))
             more = dict(lr=[x[0]["lr"] for x in items], weight_decay=[x[0]["weight_decay"] for x in items], betas=betas, eps=eps, grad_scale=coef)
             if self.state_bits == 8:
                 # (a step whose number is on the GPU adds it to the key there)
@@ -260,9 +301,7 @@ class AdamW(torch.optim.Optimizer):
         """torch.optim.AdamW's layout: {"step": fp32 tensor, "exp_avg", "exp_avg_sq": fp32} a parameter."""
         sd = super().state_dict()
         for i, st in sd["state"].items():
-            m, v = st["exp_avg"], st["exp_avg_sq"]
-            if "scales" in st:
-                m, v = state8_read(m, v, st["scales"])
+            m, v = self._averages(st)
             sd["state"][i] = {"step": torch.tensor(float(st["step"])), "exp_avg": m, "exp_avg_sq": v}
         return sd
 
@@ -280,12 +319,8 @@ class AdamW(torch.optim.Optimizer):
             if i not in states:
                 continue
             step = int(states[i]["step"])
-            m, v = (states[i][k].detach().to(device=p.device, dtype=torch.float32).reshape(p.shape).contiguous() for k in ("exp_avg", "exp_avg_sq"))
             st = self.state[p]
-            if self.state_bits == 8:
-                st["exp_avg"], st["exp_avg_sq"], st["scales"] = state8_write(m, v)
-            else:
-                st["exp_avg"], st["exp_avg_sq"] = m.clone(), v.clone()
+            self._hold(st, p, _order(p), *(states[i][k].detach().to(device=p.device, dtype=torch.float32).reshape(p.shape) for k in ("exp_avg", "exp_avg_sq")))
             st["step"] = step
             if self.capturable:
                 rule = rules[id(p)]
