@@ -240,7 +240,9 @@ class AdamW(torch.optim.Optimizer):
                 rule = (tuple(group["betas"]), group["eps"])
                 if st["step"] is None:
                     st["step"] = self._counter(fresh, (p.device,) + rule, 0, p.device) if self.capturable else 0
-                g = _flat(p.grad.resolve_neg(), order).contiguous()
+                # (a gradient that requires grad would stand for its own in grad_norm)
+                g = p.grad.detach() if p.grad.requires_grad else p.grad
+                g = _flat(g.resolve_neg(), order).contiguous()
                 grads.append(g)
                 number = id(st["step"]) if self.capturable else st["step"]
                 calls.setdefault(rule + (number,), []).append((group, p, g, st, order))
