@@ -575,7 +575,10 @@ class FlatAdamW(FlatSGD):
             raise ValueError("ODW.STATE_BITS = %r (8 | 32)" % (odw.STATE_BITS,))
         if not self.clip_norm >= 0.0:
             raise ValueError("ODW.CLIP_NORM = %r" % (odw.CLIP_NORM,))
-        self.steps = 0                  # updates taken
+        self.steps = 0                  # steps taken
+        # The head's updates beyond those: a step that fails behind head_grads_ready has moved the head's averages and parameters and nothing
+        # else.  The retried step moves them again, as the head's next update -- with its own bias correction and random bits.
+        self.head_ahead = 0
         self.grad_norm = None           # of the last step, where it was clipped (0-dim, on the GPU)
         super().__init__(cfg, model, world)
 
@@ -595,6 +598,7 @@ class FlatAdamW(FlatSGD):
             # (the norm of the mean over the ranks is the sum's over world)
             norm, self._coef = optim.grad_norm([self.flat_g], max_norm=self.clip_norm * self.world)
             self.grad_norm = norm / self.world
+        taken = self.steps + (self.head_ahead if 0 in regions else 0)
         which = [i for i in regions if self.regions[i][1] > 0]
         cut = [self.regions[i] for i in which]
         p, g = ([flat[s:s + n] for s, n, _, _ in cut] for flat in (self.flat_p, self.flat_g))
@@ -603,11 +607,13 @@ class FlatAdamW(FlatSGD):
                     grad_scale=self._coef, copies=copies, grad_mult=1.0 / self.world, max_workgroups=int(paced))
         if self.bits == 8:
             m, v, e = ([self.state8[i][k] for i in which] for k in range(3))
-            key = rng.stream_key(self.cfg.SEED & 0xFFFFFFFF, (1 << 40) + 4 * self.steps + regions[0])
-            optim.adamw8_step(p, g, m, v, e, self.steps + 1, key, **more)
+            key = rng.stream_key(self.cfg.SEED & 0xFFFFFFFF, (1 << 40) + 4 * taken + regions[0])
+            optim.adamw8_step(p, g, m, v, e, taken + 1, key, **more)
         else:
             m, v = ([flat[s:s + n] for s, n, _, _ in cut] for flat in (self.flat_m, self.flat_v))
-            optim.adamw_step(p, g, m, v, self.steps + 1, **more)
+            optim.adamw_step(p, g, m, v, taken + 1, **more)
+        if 0 in regions:
+            self.head_ahead += 1        # (until step() counts it for all)
 
     _coef = None
 
@@ -623,6 +629,7 @@ class FlatAdamW(FlatSGD):
     def step(self):
         super().step()
         self.steps += 1
+        self.head_ahead -= 1
 
     def set_iteration(self, iteration):
         self.lr_scale = lr_factor(self.cfg, iteration)
@@ -643,7 +650,7 @@ class FlatAdamW(FlatSGD):
         s = self.cfg.SOLVER
         self.join_side()
         groups, state = [], {}
-        m, v = self._averages() if self.steps > 0 else (None, None)
+        m, v = self._averages() if self.steps + self.head_ahead > 0 else (None, None)
         shapes = {n: p.shape for n, p in model.named_parameters()}
         for i, n in enumerate(self._param_order(model)):
             off, numel = self.slices[n]
@@ -651,8 +658,9 @@ class FlatAdamW(FlatSGD):
             groups.append({"lr": (s.BASE_LR * s.BIAS_LR_FACTOR if bias else s.BASE_LR) * self.lr_scale, "betas": self.betas, "eps": self.eps,
                            "weight_decay": s.WEIGHT_DECAY_BIAS if bias else s.WEIGHT_DECAY, "amsgrad": False, "maximize": False,
                            "foreach": None, "capturable": False, "differentiable": False, "fused": None, "params": [i]})
-            if self.steps > 0:
-                state[i] = {"step": torch.tensor(float(self.steps)), "exp_avg": m[off:off + numel].view(shapes[n]).clone(),
+            taken = self.steps + (self.head_ahead if off < self.n_gemm else 0)
+            if taken > 0:
+                state[i] = {"step": torch.tensor(float(taken)), "exp_avg": m[off:off + numel].view(shapes[n]).clone(),
                             "exp_avg_sq": v[off:off + numel].view(shapes[n]).clone()}
         return {"state": state, "param_groups": groups}
 
@@ -669,7 +677,7 @@ class FlatAdamW(FlatSGD):
         if any("momentum_buffer" in st for st in state.values()):
             raise ValueError("the checkpoint's optimizer state is SGD's momentum; ODW.OPTIMIZER is ADAMW")
         flat = [torch.zeros_like(self.flat_p) for _ in range(2)]
-        steps = set()
+        steps, head_steps = set(), set()
         for i, n in enumerate(order):
             entry = state.get(i, state.get(str(i)))
             if entry is None:
@@ -677,17 +685,21 @@ class FlatAdamW(FlatSGD):
             off, numel = self.slices[n]
             for f, k in zip(flat, ("exp_avg", "exp_avg_sq")):
                 f[off:off + numel].copy_(entry[k].reshape(-1).to(f.device))
-            steps.add(int(entry["step"]))
-        if not steps:
+            (head_steps if off < self.n_gemm else steps).add(int(entry["step"]))
+        if not steps and not head_steps:
             return 0
-        if len(steps) != 1:
-            raise ValueError("optimizer state: parameters have taken different numbers of steps %s" % sorted(steps))
+        if len(steps) > 1 or len(head_steps) > 1:
+            raise ValueError("optimizer state: parameters have taken different numbers of steps %s" % sorted(steps | head_steps))
         if self.bits == 8:
             for (s, n, _, _), st in zip(self.regions, self.state8):
                 optim.state8_write(flat[0][s:s + n], flat[1][s:s + n], out=st)
         else:
             self.flat_m, self.flat_v = flat
-        self.steps = steps.pop()
+        if steps or any(off >= self.n_gemm for off, _ in self.slices.values()):
+            self.steps = max(steps, default=0)
+            self.head_ahead = max(head_steps, default=self.steps) - self.steps
+        else:
+            self.steps, self.head_ahead = max(head_steps), 0
         self.first = False
         return len(state)
 
@@ -854,6 +866,7 @@ def build_training_step(cfg, device, dtype="bf16", world=1, seed=1234, backend="
             # iteration number, like the reference's trainer.py:86,118), over the micro-steps that follow the failure.
             # With the early update on (head_grads_ready), the head's SGD pass of a step that fails AFTER the pooling node's
             # backward has already been applied; a failure before that point (the fused loss, the head's backward) has not.
+            # (FlatAdamW counts it: head_ahead.)
             opt.grads_clean = True
             opt.hold = False
             for sh in opt.shadows:
