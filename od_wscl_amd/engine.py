@@ -866,7 +866,9 @@ def build_training_step(cfg, device, dtype="bf16", world=1, seed=1234, backend="
             # iteration number, like the reference's trainer.py:86,118), over the micro-steps that follow the failure.
             # With the early update on (head_grads_ready), the head's SGD pass of a step that fails AFTER the pooling node's
             # backward has already been applied; a failure before that point (the fused loss, the head's backward) has not.
-            # (FlatAdamW counts it: head_ahead.)
+            # (FlatAdamW counts it: head_ahead.)  The next forward must not read the weights while the side stream writes them.
+            if opt.side is not None:
+                torch.cuda.current_stream().wait_stream(opt.side)
             opt.grads_clean = True
             opt.hold = False
             for sh in opt.shadows:
