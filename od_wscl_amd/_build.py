@@ -41,8 +41,8 @@ def _bind_command():
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), "/opt/rocm/include"]
     return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
              "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch.compiled_with_cxx11_abi())] + [f for i in inc for f in ("-isystem", i)] +
-            ["-I" + sysconfig.get_paths()["include"], BIND_SRC, "-o", BIND, "-L" + HERE, "-l:" + os.path.basename(LIB), "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu",
-             "-ltorch", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN"])
+            ["-I" + sysconfig.get_paths()["include"], BIND_SRC, "-o", BIND, "-L" + HERE, "-l:" + os.path.basename(LIB),
+             "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN"])
 
 
 def _object(src):

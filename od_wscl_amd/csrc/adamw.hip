@@ -1,10 +1,10 @@
 // adamw.hip -- the AdamW update of many tensors in one launch (states in fp32, or in 8-bit floats with block scales), and the
 // global gradient norm it is clipped by.
 //
-// A launch takes up to kMaxTensors tensors (the norm kNormTensors): their pointers and sizes travel in the kernel's arguments (no table in device
-// memory to upload, nothing to keep alive for a captured launch).  The tensors are cut into chunks; a
-// workgroup finds the tensor of its chunk with one load of the chunks' prefix, a lane a tensor (the arguments lie in host memory: a bisection's six
-// dependent loads of them were half the time of a small launch).
+// A launch takes up to kMaxTensors tensors (the norm kNormTensors): their pointers and sizes travel in the kernel's arguments (no table
+// in device memory to upload, nothing to keep alive for a captured launch).  The tensors are cut into chunks; a workgroup finds the
+// tensor of its chunk with one load of the chunks' prefix, a lane a tensor (the arguments lie in host memory: a bisection's six dependent
+// loads of them were half the time of a small launch).
 //
 // Both are bound by the bytes: an element's update is ~20 operations on 28 bytes with fp32 states (30 with a bf16 copy of p), ~70 on 16
 // (18) with 8-bit ones.  153 M parameters in 42 tensors with copies: 796 us (5.8 TB/s) and 463 us (5.9 TB/s); their gradients' norm
@@ -18,12 +18,12 @@ namespace {
 constexpr int kMaxTensors = 48, kNormTensors = 160;      // (the arguments stay under 4 KB)
 constexpr int kBlock = 256;              // elements that share a scale: one wave, four elements a lane
 // A workgroup's four waves have a whole chunk's loads in flight: 4 blocks a wave of fp32 states, 2 of 8-bit ones (more registers a
-// block).  153 M parameters with bf16 copies, us: fp32 states 825 (2 blocks), 796 (4), 819 (8); 8-bit states 493 (1), 468 (2), 475 (4); chunks
-// of several rounds are slower (4096 elements by 2 blocks: 485; 16384: 528), and so are plain loads (522) or plain stores (511) for the
-// nontemporal ones.
+// block).  153 M parameters with bf16 copies, us: fp32 states 825 (2 blocks), 796 (4), 819 (8); 8-bit states 493 (1), 468 (2), 475 (4);
+// chunks of several rounds are slower (4096 elements by 2 blocks: 485; 16384: 528), and so are plain loads (522) or plain stores (511)
+// for the nontemporal ones.
 constexpr int unroll(bool bits8) { return bits8 ? 2 : 4; }
 constexpr int chunk_of(bool bits8) { return unroll(bits8) * 4 * kBlock; }
-constexpr int kMaxGrid = 1 << 23;        // (a launch has fewer than 2^32 threads; the update's workgroups walk on, the norm's chunks are enough)
+constexpr int kMaxGrid = 1 << 23;        // (a launch has fewer than 2^32 threads; the update's workgroups walk on)
 constexpr int kNormChunk = 16384;        // the same of the norm: fewer partial sums for the workgroup that adds them
 constexpr int kThreads = 256;
 
@@ -164,9 +164,10 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, int lane, int left, ui
 // step) instead of (grid step)^2 / 6 -- summed over v's memory of 1 / (1 - beta2) steps a standard deviation of ~0.15 of sqrt(v), without
 // a bias of v, instead of one larger than v itself.
 // A v that is not zero is held as 2^-16 of its scale at least.  An element whose gradients are far below its block's largest can have
-// its m rounded up to the smallest number, 2^-17 of the block's largest m; over a v held as zero that would be an update of any size
-// -- over 2^-32 of the block's largest v it is at most lr x a few (largest m <= 3.2 sqrt(largest v) for beta = 0.9, 0.999).  (kVToZero: v is
-// rounded to zero like any other value, without that bound.)
+// its m rounded up to the smallest number, at most 2^-16.8 of the block's largest m; over a v held as zero that would be an update of any
+// size -- over 2^-31.8 of the block's largest v, whose root is 2^-15.9 of the largest root, it is at most 4 lr: the largest m is at most
+// (1 - b1) / sqrt((1 - b2) (1 - b1^2 / b2)) = 7.3 largest roots for beta = 0.9, 0.999 (Cauchy and Schwarz on the two sums of past
+// gradients).  (kVToZero: v is rounded to zero like any other value, without that bound.)
 // All of it is integer arithmetic on the fp32 words: the same bits whatever the launch geometry.
 template <int BIAS, int MANT>
 __device__ __forceinline__ uint32_t encode8(float x, float inv_scale, uint32_t rand16, uint32_t least, bool any_bad) {
@@ -206,10 +207,11 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 
 struct Step { float gs, rc2, step, decay; uint32_t k1, least_v; };
 
-// p, g, m, v in, p, m, v (and p's bf16 copy) out, for U blocks of 256 elements `stride` apart, `left0` elements being there from the first one's start: all loads first.  The averages are formed with
-// one rounding an operation (no contraction), in the order m b1 + g (1 - b1), v b2 + g g (1 - b2); the ratio with the hardware's root and
-// reciprocal (1 ulp each: 2^-22 of a step of lr is far below p's rounding; eps keeps the reciprocal's argument above 1e-15 and makes roots
-// of subnormal numbers, which the instruction takes for zero, irrelevant).
+// p, g, m, v in, p, m, v (and p's bf16 copy) out, for U blocks of 256 elements `stride` apart, `left0` elements being there from the
+// first one's start: all loads first.  The averages are formed with one rounding an operation (no contraction), in the order m b1 + g (1
+// - b1), v b2 + g g (1 - b2); the ratio with the hardware's root and reciprocal (1 ulp each: 2^-22 of a step of lr is far below p's
+// rounding; eps keeps the reciprocal's argument above 1e-15 and makes roots of subnormal numbers, which the instruction takes for zero,
+// irrelevant).
 template <bool BITS8, bool PBF, bool GBF, bool FULL, int U>
 __device__ __forceinline__ void update(const Args& a, const Tensor& t, const Step& s, int64_t base, int stride, int lane, int left0) {
     Four<PBF, FULL> p[U];
@@ -294,8 +296,8 @@ __device__ __forceinline__ void update(const Args& a, const Tensor& t, const Ste
     }
 }
 
-// A chunk: its four waves take every fourth block, all at once -- a tensor's last, short chunk as well, whose blocks one after the other would
-// cost small tensors a round trip to memory each.
+// A chunk: its four waves take every fourth block, all at once -- a tensor's last, short chunk as well, whose blocks one after the other
+// would cost small tensors a round trip to memory each.
 template <bool BITS8, bool PBF, bool GBF>
 __device__ __forceinline__ void chunk(const Args& a, const Tensor& t, const Step& s, int64_t begin, int wave, int lane) {
     constexpr int kWaves = kThreads / 64;
@@ -363,7 +365,8 @@ __device__ __forceinline__ double sqsum(const void* g, int size, int wave, int l
     for (; b * kBlock < size; b += U * kWaves) {
         Four<BF, false> x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u].load((const char*)g + (size_t)(b + u * kWaves) * kBlock * (BF ? 2 : 4), lane, size - (b + u * kWaves) * kBlock);
+        for (int u = 0; u < U; ++u)
+            x[u].load((const char*)g + (size_t)(b + u * kWaves) * kBlock * (BF ? 2 : 4), lane, size - (b + u * kWaves) * kBlock);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll

@@ -1,10 +1,11 @@
-// bind.cpp -- torch-side glue of the optimiser and the row norm (od_wscl_amd/_bind.so): argument checks over tensor lists, workspaces, and the
-// norm's autograd node, in front of the C-ABI of libodwscl.so.
+// bind.cpp -- torch-side glue of the optimiser and the row norm (od_wscl_amd/_bind.so): argument checks over tensor lists, workspaces,
+// and the norm's autograd node, in front of the C-ABI of libodwscl.so.
 //
-// The other operators are bound by ctypes; these are called with lists of a hundred small tensors, or once a layer on a few rows, where Python's
-// look at each tensor (0.35 us for its device, type, size, layout and address) and the autograd engine's way through Python were the time of the
-// call.  From Python / from here, us: 8-bit AdamW over 120 tensors 197 / 37 (its kernels 28), clipping 16 tensors 28 / 17, the norm of one row
-// 13.4 / 6.5, forward and backward of 447 x 1373 117 / 57.  No kernel lives here.
+// The other operators are bound by ctypes; these are called with lists of a hundred small tensors, or once a layer on a few rows, where
+// Python's look at each tensor (0.35 us for its device, type, size, layout and address) was most of the call.  From Python / from here,
+// us: 8-bit AdamW over 120 tensors 200 / 38 (its kernels 28), clipping 16 tensors 29 / 17.5, the norm of one row 13.7 / 6.8, forward and
+// backward of 447 x 1373 53 to 108 / 58 to 60 (the autograd engine hands over to its own thread: 33 for a node without a kernel).  No
+// kernel lives here.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -49,7 +50,8 @@ std::string format(const char* fmt, va_list ap) {
 void need_gpu(const Tensor& t) {
     if (!t.is_cuda()) throw std::runtime_error("od_wscl_amd: tensor is not on the GPU -- the hot path has no CPU implementation");
     // (the stand-ins of torch.func's transforms)
-    if (t.layout() == at::kStrided && !t.has_storage()) throw std::runtime_error("od_wscl_amd: tensor has no memory of its own -- a transform's stand-in");
+    if (t.layout() == at::kStrided && !t.has_storage())
+        throw std::runtime_error("od_wscl_amd: tensor has no memory of its own -- a transform's stand-in");
 }
 void check(int code, const char* what) {
     if (code != 0) throw std::runtime_error(std::string(what) + " failed (" + std::to_string(code) + "): " + odw_last_error());
@@ -77,9 +79,9 @@ std::string names_of(const Types& types) {
     return s;
 }
 
-// `list` beside the first one: as many, on its GPU, contiguous, of one of `types` and of `sizes`; their addresses.  What is written must not be in
-// a list twice (two workgroups would update it at once).  `alone` (a norm, a scaling): elements go with no other list's, so that any order without
-// gaps will do, and a lazily negated view too, whose memory holds the other sign.
+// `list` beside the first one: as many, on its GPU, contiguous, of one of `types` and of `sizes`; their addresses.  What is written must
+// not be in a list twice (two workgroups would update it at once).  `alone` (a norm, a scaling): elements go with no other list's, so
+// that any order without gaps will do, and a lazily negated view too, whose memory holds the other sign.
 std::vector<void*> addresses(const char* what, const char* name, const std::vector<Tensor>& list, int device, const std::vector<int64_t>& sizes,
                              const Types& types, bool written, bool alone = false) {
     if (list.size() != sizes.size()) value_error("%s: %zu %s for %zu tensors", what, list.size(), name, sizes.size());
@@ -88,13 +90,15 @@ std::vector<void*> addresses(const char* what, const char* name, const std::vect
     for (size_t i = 0; i < list.size(); ++i) {
         const Tensor& t = list[i];
         need_gpu(t);
-        if (t.get_device() != device) value_error("%s: %s[%zu] is on cuda:%d, tensor 0 on cuda:%d", what, name, i, (int)t.get_device(), device);
+        if (t.get_device() != device)
+            value_error("%s: %s[%zu] is on cuda:%d, tensor 0 on cuda:%d", what, name, i, (int)t.get_device(), device);
         bool known = false;
         for (at::ScalarType k : types) known |= t.scalar_type() == k;
         if (!known || t.layout() != at::kStrided)
             type_error("%s: %s[%zu] is %s%s (%s)", what, name, i, t.layout() != at::kStrided ? "sparse " : "", name_of(t.scalar_type()).c_str(),
                        names_of(types).c_str());
-        if (t.numel() != sizes[i]) value_error("%s: %s[%zu] has %lld elements, %lld wanted", what, name, i, (long long)t.numel(), (long long)sizes[i]);
+        if (t.numel() != sizes[i])
+            value_error("%s: %s[%zu] has %lld elements, %lld wanted", what, name, i, (long long)t.numel(), (long long)sizes[i]);
         if (alone ? !t.is_non_overlapping_and_dense() : !t.is_contiguous()) value_error("%s: %s[%zu] is not contiguous", what, name, i);
         if (!alone && t.is_neg()) value_error("%s: %s[%zu] is a negated view (resolve_neg)", what, name, i);
         at.push_back(t.numel() ? t.data_ptr() : nullptr);
@@ -197,13 +201,15 @@ void adamw(bool bits8, const std::vector<Tensor>& params, const std::vector<Tens
     const char* what = bits8 ? "adamw8_step" : "adamw_step";
     not_traced(what);
     const at::NoGradGuard no_grad;
-    if (bits8 && (key.size() != 2 || key[0] < 0 || key[1] < 0 || key[0] >> 32 || key[1] >> 32)) value_error("%s: key has to be two 32-bit integers", what);
+    if (bits8 && (key.size() != 2 || key[0] < 0 || key[1] < 0 || key[0] >> 32 || key[1] >> 32))
+        value_error("%s: key has to be two 32-bit integers", what);
     if (params.empty()) return;
     need_gpu(params[0]);
     const int device = params[0].get_device();
     const size_t count = params.size();
     const std::vector<int64_t> n = sizes_of(params);
-    const std::vector<void*> ap = addresses(what, "params", params, device, n, kFloats, true), ag = addresses(what, "grads", grads, device, n, kFloats, false),
+    const std::vector<void*> ap = addresses(what, "params", params, device, n, kFloats, true),
+                             ag = addresses(what, "grads", grads, device, n, kFloats, false),
                              am = addresses(what, "exp_avgs", m, device, n, {bits8 ? at::kFloat8_e4m3fn : at::kFloat}, true),
                              av = addresses(what, "exp_avg_sqs", v, device, n, {bits8 ? at::kFloat8_e5m2 : at::kFloat}, true);
     std::vector<void*> ae, ac;
@@ -226,7 +232,8 @@ void adamw(bool bits8, const std::vector<Tensor>& params, const std::vector<Tens
         size_t j = 0;
         for (size_t i = 0; i < count; ++i) ac.push_back((*copies)[i] ? at[j++] : nullptr);
     }
-    if (betas.size() != 2 || !(betas[0] >= 0.0 && betas[0] < 1.0) || !(betas[1] >= 0.0 && betas[1] < 1.0)) value_error("%s: betas have to be two numbers in [0, 1)", what);
+    if (betas.size() != 2 || !(betas[0] >= 0.0 && betas[0] < 1.0) || !(betas[1] >= 0.0 && betas[1] < 1.0))
+        value_error("%s: betas have to be two numbers in [0, 1)", what);
     // (a gradient whose square is nothing in fp32, below 1e-21, then moves p by at most lr * 1e-6, not by lr * g / eps of any size)
     if (!(eps >= 1e-15 && std::isfinite((float)eps))) value_error("%s: eps = %g", what, eps);
     if (!std::isfinite((float)grad_mult)) value_error("%s: grad_mult = %g", what, grad_mult);
@@ -235,7 +242,9 @@ void adamw(bool bits8, const std::vector<Tensor>& params, const std::vector<Tens
     const std::vector<float> lrs = scalars(what, "lr", lr, count), wds = scalars(what, "weight_decay", weight_decay, count);
     if (grad_scale) device_scalar(what, "grad_scale", *grad_scale, device, at::kFloat);
     std::vector<int> types;
-    for (size_t i = 0; i < count; ++i) types.push_back((params[i].scalar_type() == at::kBFloat16 ? 1 : 0) + (grads[i].scalar_type() == at::kBFloat16 ? 2 : 0) + (bits8 && !hold_v ? 4 : 0));
+    for (size_t i = 0; i < count; ++i)
+        types.push_back((params[i].scalar_type() == at::kBFloat16 ? 1 : 0) + (grads[i].scalar_type() == at::kBFloat16 ? 2 : 0) +
+                        (bits8 && !hold_v ? 4 : 0));
     const c10::DeviceGuard guard(params[0].device());
     void* stream = stream_of(params[0]);
     Tensor bias;
@@ -286,35 +295,44 @@ void check_rows(const char* what, const Tensor& x, const OptTensor& weight, cons
     need_gpu(x);
     if (x.dim() < 1 || x.size(-1) < 1) value_error("%s: x has no columns", what);
     if (x.size(-1) > INT32_MAX) value_error("%s: x has %lld columns", what, (long long)x.size(-1));
-    const std::pair<const char*, const Tensor*> all[3] = {{"x", &x}, {"weight", weight ? &*weight : nullptr}, {"residual", residual ? &*residual : nullptr}};
+    const std::pair<const char*, const Tensor*> all[3] = {
+        {"x", &x}, {"weight", weight ? &*weight : nullptr}, {"residual", residual ? &*residual : nullptr}};
     for (const auto& [name, t] : all) {
         if (!t) continue;
         need_gpu(*t);
         if (t->scalar_type() != at::kFloat && t->scalar_type() != at::kBFloat16)
             type_error("%s: %s is %s (torch.float32 | torch.bfloat16)", what, name, name_of(t->scalar_type()).c_str());
-        if (t->get_device() != x.get_device()) value_error("%s: %s is on cuda:%d, x on cuda:%d", what, name, (int)t->get_device(), (int)x.get_device());
+        if (t->get_device() != x.get_device())
+            value_error("%s: %s is on cuda:%d, x on cuda:%d", what, name, (int)t->get_device(), (int)x.get_device());
     }
     if (weight && (weight->dim() != 1 || weight->size(0) != x.size(-1)))
-        value_error("%s: weight has %lld elements in %lld dimensions, x %lld columns", what, (long long)weight->numel(), (long long)weight->dim(), (long long)x.size(-1));
+        value_error("%s: weight has %lld elements in %lld dimensions, x %lld columns", what, (long long)weight->numel(),
+                    (long long)weight->dim(), (long long)x.size(-1));
     if (residual && residual->sizes() != x.sizes()) value_error("%s: residual has another shape than x", what);
     if (residual && residual->scalar_type() != x.scalar_type() && residual->scalar_type() != at::kFloat)
-        type_error("%s: residual is %s beside x in %s (x's type or torch.float32)", what, name_of(residual->scalar_type()).c_str(), name_of(x.scalar_type()).c_str());
+        type_error("%s: residual is %s beside x in %s (x's type or torch.float32)", what, name_of(residual->scalar_type()).c_str(),
+                   name_of(x.scalar_type()).c_str());
     if (!(eps >= 0.0 && std::isfinite((float)eps))) value_error("%s: eps = %g", what, eps);
 }
 
-int types_of(at::ScalarType x, at::ScalarType h, const Tensor& w) { return is_bf16(x) + 2 * is_bf16(h) + (w.defined() && is_bf16(w.scalar_type()) ? 4 : 0); }
+int types_of(at::ScalarType x, at::ScalarType h, const Tensor& w) {
+    return is_bf16(x) + 2 * is_bf16(h) + (w.defined() && is_bf16(w.scalar_type()) ? 4 : 0);
+}
 
 // The forward launch into `out` (y, or with `scale` the 8-bit codes); h is undefined without a residual.
-Tensor norm_rows(const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps, const Tensor& out, const Tensor& rstd, const Tensor& scale) {
+Tensor norm_rows(const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps, const Tensor& out, const Tensor& rstd,
+                 const Tensor& scale) {
     const int64_t D = x.size(-1);
     const Tensor x2 = rows(x, D), r2 = residual ? rows(*residual, D) : Tensor(), w = weight ? weight->resolve_neg().contiguous() : Tensor();
     const Tensor h = residual ? at::empty(x.sizes(), residual->options()) : Tensor();
     const int types = types_of(x.scalar_type(), (residual ? *residual : x).scalar_type(), w);
     const int64_t R = x2.size(0), ldx = x2.stride(0), ldr = residual ? r2.stride(0) : 0;
     if (scale.defined())
-        check(odw_rms_norm_fp8(ptr(x2), ldx, ptr(r2), ldr, ptr(w), R, (int)D, (float)eps, ptr(out), (float*)ptr(scale), ptr(h), types, stream_of(x)), "rms_norm_fp8");
+        check(odw_rms_norm_fp8(ptr(x2), ldx, ptr(r2), ldr, ptr(w), R, (int)D, (float)eps, ptr(out), (float*)ptr(scale), ptr(h), types,
+                               stream_of(x)), "rms_norm_fp8");
     else
-        check(odw_rms_norm(ptr(x2), ldx, ptr(r2), ldr, ptr(w), R, (int)D, (float)eps, ptr(out), ptr(h), (float*)ptr(rstd), types, stream_of(x)), "rms_norm");
+        check(odw_rms_norm(ptr(x2), ldx, ptr(r2), ldr, ptr(w), R, (int)D, (float)eps, ptr(out), ptr(h), (float*)ptr(rstd), types,
+                           stream_of(x)), "rms_norm");
     return h;
 }
 
@@ -324,7 +342,8 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& residual,
                                                   double eps) {
         const c10::DeviceGuard guard(x.device());
-        const Tensor y = at::empty(x.sizes(), x.options()), rstd = at::empty({x.numel() / x.size(-1)}, x.options().dtype(at::kFloat));
+        const Tensor y = at::empty(x.sizes(), x.options()),
+                     rstd = at::empty({x.numel() / x.size(-1)}, x.options().dtype(at::kFloat));
         const Tensor h = norm_rows(x, weight, residual, eps, y, rstd, Tensor());
         ctx->save_for_backward({h.defined() ? h : x, weight ? *weight : Tensor(), rstd});
         ctx->set_materialize_grads(false);
@@ -353,7 +372,8 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
         return {out[0], out[1], out[2], Tensor()};
     }
 
-    static torch::autograd::variable_list gradients(int64_t flags, const Tensor& h, const Tensor& weight, const Tensor& rstd, const Tensor& dy, const Tensor& dh) {
+    static torch::autograd::variable_list gradients(int64_t flags, const Tensor& h, const Tensor& weight, const Tensor& rstd,
+                                                    const Tensor& dy, const Tensor& dh) {
         const bool need_x = flags & kNeedX, need_w = flags & kNeedW, need_r = flags & kNeedR;
         const at::ScalarType x_type = flags & kXIsBf16 ? at::kBFloat16 : at::kFloat, h_type = flags & kHasR ? h.scalar_type() : x_type;
         if (!dy.defined()) {             // only h was used
@@ -361,7 +381,8 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
         }
         const c10::DeviceGuard guard(h.device());
         const int64_t D = h.size(-1);
-        const Tensor h2 = rows(h, D), g2 = rows(dy, D), d2 = dh.defined() ? rows(dh, D) : Tensor(), w = weight.defined() ? weight.resolve_neg().contiguous() : Tensor();
+        const Tensor h2 = rows(h, D), g2 = rows(dy, D), d2 = dh.defined() ? rows(dh, D) : Tensor(),
+                     w = weight.defined() ? weight.resolve_neg().contiguous() : Tensor();
         const int64_t R = h2.size(0);
         const bool mixed = h_type != x_type;
         const Tensor dx = need_x || (need_r && !mixed) ? at::empty(h.sizes(), h.options().dtype(x_type)) : Tensor();
@@ -394,7 +415,8 @@ py::object rms_norm_fp8(const Tensor& x, const OptTensor& weight, const OptTenso
     const at::NoGradGuard no_grad;
     check_rows("rms_norm_fp8", x, weight, residual, eps);
     const c10::DeviceGuard guard(x.device());
-    const Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    const Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)),
+                 scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
     const Tensor h = norm_rows(x, weight, residual, eps, q, Tensor(), scale);
     return residual ? py::make_tuple(q, scale, h) : py::make_tuple(q, scale);
 }

@@ -11,9 +11,11 @@ namespace {
 
 enum { kXBf16 = 1, kHBf16 = 2, kWBf16 = 4 };
 
-// Outputs of the forward pass over this many bytes (the eight L2s together) are stored past the caches (PAST): nothing of them would be left
-// there for the next kernel, and the rows coming in keep their place.  2000 x 4096 fp32 with residual 27.7 us -> 20.1 (6.5 TB/s),
-// 16000 x 4096 bf16 96 -> 91.  (Loads past the caches: 30 and 106; stores of the backward pass: no difference.)
+// Outputs of the forward pass over this many bytes (the eight L2s together) are stored past the caches (PAST): nothing of them would be
+// left there for the next kernel, and the rows coming in keep their place.  Calls one after the other on three sets of rows in turn, us:
+// 2000 x 4096 fp32 with residual 23.9 -> 20.0 (6.6 TB/s), 16000 x 4096 bf16 96.1 -> 91.4; forward and backward 201 -> 195.  (A launch by
+// itself, as in a trace, is a little slower with it: 24.4 -> 26.0 and 93.5 -> 98.2.  Loads past the caches: slower; stores of the
+// backward pass: no difference.)
 constexpr int64_t kL2Bytes = (int64_t)32 << 20;
 
 __device__ __forceinline__ float ld(const void* p, bool bf, int64_t i) {
@@ -59,11 +61,11 @@ __device__ __forceinline__ uint32_t block_max(uint32_t x, uint32_t* part) {
 __device__ __forceinline__ uint8_t to_e4m3(float x) { return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false); }
 
 // ---- rows that fit the registers ------------------------------------------------------------------------------------------------
-// TPR threads hold a row, VPT vectors of V elements each (16 bytes of x's type): one pass over memory, and between load and store the row's sum (and largest word) over the lanes -- by
-// cross-lane moves for TPR = 64, through LDS beyond.  Rows of any pitch, width and alignment go the
-// same way (the vector loads and stores are declared with their element's alignment, which the memory instructions take as well; a row's
-// last, short vector goes by elements): a row's result does not depend on where it lies.  The forms differ in TX (x, y, dy, dx) and TH (residual, h, dh, dresidual); the rest is
-// uniform branches.
+// TPR threads hold a row, VPT vectors of V elements each (16 bytes of x's type): one pass over memory, and between load and store the
+// row's sum (and largest word) over the lanes -- by cross-lane moves for TPR = 64, through LDS beyond.  Rows of any pitch, width and
+// alignment go the same way (the vector loads and stores are declared with their element's alignment, which the memory instructions take
+// as well; a row's last, short vector goes by elements): a row's result does not depend on where it lies.  The forms differ in TX (x, y,
+// dy, dx) and TH (residual, h, dh, dresidual); the rest is uniform branches.
 
 template <class T, int V> struct Vec {
     typedef T full __attribute__((ext_vector_type(V)));
@@ -152,12 +154,12 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x, float* part) {
     return x;
 }
 
-// The 8-bit codes are the correctly rounded ones, q = rne(y / (max |y| / 448)), where a quotient rounded to fp32 on the way would go the other
-// way round a few times in a million.  The row's factor cancels in it: with t = h w, q = rne(448 t / max |t|).  The fp32 quotient z stands for
-// an interval; a thread rounds both its ends, and only rows with a code that is open then go the long way for those codes: t = p + e
-// exactly (p the rounded product, e its error by one fma), 448 / max |t| = c + cl in two fp32 numbers, and the product's first 24 bits in f,
-// the rest in the sign of lo: f with its last bit standing for "and something more" (rounding to odd) rounds to 8 bits as the exact product.
-// (Every element the long way: 2000 x 25088 fp32 76 us.)
+// The 8-bit codes are the correctly rounded ones, q = rne(y / (max |y| / 448)), where a quotient rounded to fp32 on the way would go the
+// other way round a few times in a million.  The row's factor cancels in it: with t = h w, q = rne(448 t / max |t|).  The fp32 quotient z
+// stands for an interval; a thread rounds both its ends, and only rows with a code that is open then go the long way for those codes: t =
+// p + e exactly (p the rounded product, e its error by one fma), 448 / max |t| = c + cl in two fp32 numbers, and the product's first 24
+// bits in f, the rest in the sign of lo: f with its last bit standing for "and something more" (rounding to odd) rounds to 8 bits as the
+// exact product. (Every element the long way: 2000 x 25088 fp32 76 us, for 64.)
 __device__ __forceinline__ float times_to_odd(float h, float w, float c, float cl) {
     const float p = h * w, e = fmaf(h, w, -p), z = p * c;
     const float r = fmaf(e, c, fmaf(p, cl, fmaf(p, c, -z)));
@@ -181,13 +183,13 @@ __device__ __forceinline__ void store_codes(uint8_t* q, int left, int u) {
     }
 }
 
-// OUT8: `scale` is given and y are the codes.  (The branch on `scale` is uniform and decided by OUT8; left to run time it keeps what belongs to a
-// vector together -- without it the scheduler loads the whole row's weight ahead: 2000 x 25088 bf16 92 us for 78, its registers spilt.)
+// OUT8: `scale` is given and y are the codes.  (The branch on `scale` is uniform and decided by OUT8; left to run time it keeps what
+// belongs to a vector together -- without it the scheduler loads the whole row's weight ahead: 2000 x 25088 bf16 with residual 92
+// us for 78, its registers spilt.)
 template <class TX, class TH, int TPR, int VPT, int V, bool PAST, bool OUT8>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1) void rms_norm_row_kernel(const TX* __restrict__ x, int64_t ldx, const TH* __restrict__ res,
-                                                                             int64_t ldr, const void* __restrict__ w, int64_t R, int D, float eps,
-                                                                             void* __restrict__ y, TH* h, float* __restrict__ rstd,
-                                                                             float* __restrict__ scale, int types) {
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1)
+void rms_norm_row_kernel(const TX* __restrict__ x, int64_t ldx, const TH* __restrict__ res, int64_t ldr, const void* __restrict__ w, int64_t R,
+                         int D, float eps, void* __restrict__ y, TH* h, float* __restrict__ rstd, float* __restrict__ scale, int types) {
     constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
     __shared__ float part[2][TPR > 64 ? TPR / 64 : 1];
     __shared__ int any[TPR > 64 ? TPR / 64 : 1];
@@ -287,9 +289,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1) void rms_
     // (the values again, from where they came: their registers hold the products)
     auto value = [&](int i) { return res ? up(h[r * D + i]) : up(x[r * ldx + i]); };
     auto gain = [&](int i) { return w ? ld(w, types & kWBf16, i) : 1.0f; };
-    // e of the largest product (of equal ones, in this thread and over the threads, the largest e), as a word that grows with it.  The thread
-    // that holds it loads its elements again: looked for in v they would stay in registers until here, and the widest forms spill (2000 x
-    // 25088 fp32 69-71 us for 64)
+    // e of the largest product (of equal ones, in this thread and over the threads, the largest e), as a word that grows with it.  The
+    // thread that holds it loads its elements again: looked for in v they would stay in registers until here, and the widest forms spill
+    // (2000 x 25088 fp32 69-71 us for 64)
     uint32_t key = 0;
     if (best == __float_as_uint(pm)) {
 #pragma clang loop unroll_count(2)
@@ -325,18 +327,17 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 8 : 1) void rms_
 }
 
 // Rows blockIdx.x, + gridDim.x, ... of a workgroup (TPR = 64: of each of its four waves); the weight's gradient of those rows stays in
-// registers and ends in a row of part_w of its own, which rms_norm_dw_kernel sums in order.  While a row's sum goes round, the loads of the next
-// row are in flight (kAhead): few groups of rows (little part_w) keep the memory busy.  1024 threads have half the registers each: rows over
-// 8 elements a thread are loaded when they are due there, and of the widest ones the weight's gradient lies in LDS (each thread its own
-// columns).
+// registers and ends in a row of part_w of its own, which rms_norm_dw_kernel sums in order.  While a row's sum goes round, the loads of
+// the next row are in flight (kAhead): few groups of rows (little part_w) keep the memory busy.  1024 threads have half the registers
+// each: rows over 8 elements a thread are loaded when they are due there, and of the widest ones the weight's gradient lies in LDS (each
+// thread its own columns).
 constexpr bool wide_row(int tpr, int vpt, int v) { return tpr == 1024 && vpt * v >= 32; }
 
 template <class TX, class TH, int TPR, int VPT, int V>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_row_kernel(const TX* __restrict__ dy, int64_t ldy, const TH* __restrict__ dh,
-                                                                                 int64_t ldh, const TH* __restrict__ h, int64_t ldx,
-                                                                                 const void* __restrict__ w, const float* __restrict__ rstd, int64_t R,
-                                                                                 int D, TX* __restrict__ dx, TH* __restrict__ dres,
-                                                                                 float* __restrict__ part_w, int types) {
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256)
+void rms_norm_bwd_row_kernel(const TX* __restrict__ dy, int64_t ldy, const TH* __restrict__ dh, int64_t ldh, const TH* __restrict__ h,
+                             int64_t ldx, const void* __restrict__ w, const float* __restrict__ rstd, int64_t R, int D, TX* __restrict__ dx,
+                             TH* __restrict__ dres, float* __restrict__ part_w, int types) {
     constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
     constexpr bool kWide = wide_row(TPR, VPT, V), kAhead = TPR <= 256 || VPT * V <= 8;
     __shared__ float part[2][TPR > 64 ? TPR / 64 : 1];
@@ -528,11 +529,11 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(const void* dy, int64
 template <int T_, int K_, int V_> struct Shape { static constexpr int tpr = T_, vpt = K_, v = V_; };
 template <class... S> struct Shapes {};
 
-// Rows by width, the first that holds one: a wave a row while a lane needs one or two vectors (no barrier), then 256 and 1024 threads.  16000 x
-// 1024 fp32 with a wave and four vectors a lane 49.1 us, with 256 threads 45.7; 4000 x 8192 bf16 with 256 threads and four vectors 53.7,
-// with 1024 threads 52.0.  1024 threads of up to 64 registers leave room for a second row on a compute unit: 2000 x 25088 fp32 to
-// 8 bits 72 us with one row, 56 with two.  The backward pass keeps three numbers an element (gradient, h, the weight's gradient)
-// instead of one: fewer elements a thread.
+// Rows by width, the first that holds one: a wave a row while a lane needs one or two vectors (no barrier), then 256 and 1024 threads.
+// 16000 x 1024 fp32 with a wave and four vectors a lane 49.1 us, with 256 threads 45.7; 4000 x 8192 bf16 with 256 threads and four
+// vectors 53.7, with 1024 threads 52.0.  1024 threads of up to 64 registers leave room for a second row on a compute unit: 2000 x 25088
+// fp32 to 8 bits 72 us with one row, 56 with two (64 since every code is certain).  The backward pass keeps three numbers an element
+// (gradient, h, the weight's gradient) instead of one: fewer elements a thread.
 typedef Shapes<Shape<64, 1, 4>, Shape<64, 2, 4>, Shape<256, 1, 4>, Shape<256, 2, 4>, Shape<256, 4, 4>, Shape<256, 8, 4>, Shape<1024, 4, 4>,
                Shape<1024, 5, 4>, Shape<1024, 6, 4>, Shape<1024, 7, 4>, Shape<1024, 8, 4>> Fwd4;
 typedef Shapes<Shape<64, 1, 8>, Shape<64, 2, 8>, Shape<256, 1, 8>, Shape<256, 2, 8>, Shape<1024, 1, 8>, Shape<1024, 2, 8>, Shape<1024, 4, 8>> Fwd8;
@@ -546,9 +547,9 @@ bool with_shape(int D, Shapes<S...>, F f) {
     return ((D <= S::tpr * S::vpt * S::v ? (f(S()), true) : false) || ...);
 }
 
-// Row groups of the backward pass = rows of part_w: enough to fill the chip, few beside the rows.  Measured, us: 16000 x 4096 bf16 (256 threads
-// a row) 512 groups 101, 768 107, 1024 123; 40000 x 512 bf16 (a wave a row) 1024 groups 66, 2048 45, 4096 49; 3000 x 128 fp32 1024 groups
-// 10, 2048 13.
+// Row groups of the backward pass = rows of part_w: enough to fill the chip, few beside the rows.  Measured, us: 16000 x 4096 bf16 (256
+// threads a row) 512 groups 101, 768 107, 1024 123; 40000 x 512 bf16 (a wave a row) 1024 groups 66, 2048 45, 4096 49; 3000 x 128 fp32
+// 1024 groups 10, 2048 13.
 int bwd_groups(int64_t R, int D) {
     if (D <= 1024) return (int)(R < 64 ? R : R < 8192 ? (R + 3) / 4 : 2048);        // (waves)
     const int most = D <= 4096 ? 512 : 256;

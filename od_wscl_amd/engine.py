@@ -901,5 +901,6 @@ def build_training_step(cfg, device, dtype="bf16", world=1, seed=1234, backend="
     step.model, step.optimizer = model, opt
     mode = precision.get_precision()
     info = {"gemm_backend": "od_wscl_amd HIP MFMA gemm_nt_bf16 (%s operands, fp32 acc)" % mode,
-            "conv_backend": conv_desc + " " + mode, "optimizer": "od_wscl_amd fused flat " + ("AdamW, %d-bit states" % opt.bits if isinstance(opt, FlatAdamW) else "SGD"), "precision": mode}
+            "conv_backend": conv_desc + " " + mode, "precision": mode,
+            "optimizer": "od_wscl_amd fused flat " + ("AdamW, %d-bit states" % opt.bits if isinstance(opt, FlatAdamW) else "SGD")}
     return step, info

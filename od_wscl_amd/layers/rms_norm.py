@@ -1,6 +1,6 @@
 """Root-mean-square norm over the last axis, with the residual's addition and its gradients, and its 8-bit output
-(csrc/rms_norm.hip; the autograd node: csrc/bind.cpp).  Beside FrozenBatchNorm2d (statistics of maps) and the embeddings' L2 norm (sim_head/sim_net.py): the norm of
-activation rows, for heads of one's own between layers.linear.Linear layers.  No reference counterpart."""
+(csrc/rms_norm.hip; the autograd node: csrc/bind.cpp).  Beside FrozenBatchNorm2d (statistics of maps) and the embeddings' L2 norm
+(sim_head/sim_net.py): the norm of activation rows, for heads of one's own between layers.linear.Linear layers.  No reference counterpart."""
 import torch
 from torch import nn
 
@@ -20,7 +20,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
 def rms_norm_fp8(x, weight=None, residual=None, eps=1e-6):
     """rms_norm with its output in 8 bits: (q, scale), or (q, scale, h) with a residual.  q float8_e4m3fn of x's shape, scale fp32 (...,):
     y ~ q.float() * scale[..., None], scale = max |y| / 448 of the row (2^-126 for a row of zeros).  q is the quotient correctly
-    rounded (ties to even); in rows over 32768 elements it is rounded to fp32 first.  A row that holds a NaN is all NaN.  No gradients."""
+    rounded (ties to even); it is rounded to fp32 first in rows over 32768 elements, in rows whose largest |h weight| is not between
+    1e-30 and 1e30, and where 2^-126 is the scale.  A row that holds a NaN is all NaN.  No gradients."""
     return L.bind().rms_norm_fp8(x, weight, residual, eps)
 
 

@@ -38,8 +38,9 @@ def grad_norm(grads, max_norm=None):
 
 
 def clip_grad_norm_(grads, max_norm):
-    """Scale all of `grads` (tensors, or parameters that stand for their .grad; or one) in place so that their common 2-norm is at most
-    max_norm (their elements in any order without gaps); returns the norm before that, 0 where none has a gradient (torch.nn.utils.clip_grad_norm_, without a host read)."""
+    """Scale all of `grads` (tensors, or parameters that stand for their .grad; or one; elements in any order without gaps) in place so that
+    their common 2-norm is at most max_norm; returns the norm before that, 0 where none has a gradient (torch.nn.utils.clip_grad_norm_,
+    without a host read)."""
     return L.bind().clip_grad_norm(_list(grads), max_norm)
 
 
@@ -73,8 +74,8 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, scales, step, key, lr=1e-3
 
     hold_v: a second average that is not zero is held as 2^-16 of its scale at least, which bounds the steps of elements far below their block's
     largest.  False: it is rounded to zero like any other value, and such an element may move by lr times its first average over eps."""
-    L.bind().adamw(True, params, grads, exp_avgs, exp_avg_sqs, scales, step, key, lr, betas, eps, weight_decay, grad_scale, copies, grad_mult,
-                   max_workgroups, hold_v)
+    L.bind().adamw(True, params, grads, exp_avgs, exp_avg_sqs, scales, step, key, lr, betas, eps, weight_decay, grad_scale, copies,
+                   grad_mult, max_workgroups, hold_v)
 
 
 # ---- the 8-bit states as tensors -----------------------------------------------------------------------------------------------------
@@ -259,7 +260,8 @@ class AdamW(torch.optim.Optimizer):
                 step += 1
             ps, gs = [_flat(x[1], x[4]) for x in items], [x[2] for x in items]
             m, v = ([_flat(x[3][k], x[4]) for x in items] for k in ("exp_avg", "exp_avg_sq"))
-            more = dict(lr=[x[0]["lr"] for x in items], weight_decay=[x[0]["weight_decay"] for x in items], betas=betas, eps=eps, grad_scale=coef)
+            lr, wd = ([x[0][k] for x in items] for k in ("lr", "weight_decay"))
+            more = dict(lr=lr, weight_decay=wd, betas=betas, eps=eps, grad_scale=coef)
             if self.state_bits == 8:
                 # (a step whose number is on the GPU adds it to the key there)
                 key = rng.stream_key(self.seed, (ci << 40) + (0 if self.capturable else step))
@@ -292,8 +294,8 @@ class AdamW(torch.optim.Optimizer):
             if id(st.get("step")) in taken and id(p) not in stepped:
                 apart.setdefault(("rest", id(st["step"])), (st["step"], []))[1].append(st)
         if apart and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW: parameters that share a step counter part in a captured step (other betas or eps, or a missing gradient): take "
-                               "such a step before the capture")
+            raise RuntimeError("AdamW: parameters that share a step counter part in a captured step (other betas or eps, or a missing "
+                               "gradient): take such a step before the capture")
         for counter, states in apart.values():
             own = counter.clone()
             for st in states:
@@ -322,7 +324,8 @@ class AdamW(torch.optim.Optimizer):
                 continue
             step = int(states[i]["step"])
             st = self.state[p]
-            self._hold(st, p, _order(p), *(states[i][k].detach().to(device=p.device, dtype=torch.float32).reshape(p.shape) for k in ("exp_avg", "exp_avg_sq")))
+            m, v = (states[i][k].detach().to(device=p.device, dtype=torch.float32).reshape(p.shape) for k in ("exp_avg", "exp_avg_sq"))
+            self._hold(st, p, _order(p), m, v)
             st["step"] = step
             if self.capturable:
                 rule = rules[id(p)]
