@@ -336,6 +336,23 @@ Tensor norm_rows(const Tensor& x, const OptTensor& weight, const OptTensor& resi
     return h;
 }
 
+// A captured backward pass hands its gradients on: to a leaf's accumulator that an eager graph, still alive, has made on the default
+// stream (or to any node of that stream), the engine would make that stream wait for the capture, which it cannot, and the process ends.
+// Refused before it does.
+void no_default_stream_behind_a_capture() {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+        const auto& edge = node->next_edge(i);
+        if (!edge.is_valid() || !node->task_should_compute_output(i)) continue;
+        const auto stream = edge.function->stream();
+        if (stream && stream->id() == 0)
+            throw std::runtime_error("rms_norm: a captured backward pass would reach a node of the default stream: a graph made there before, of the "
+                                     "same leaves or of the input, is still alive (let it go, or make it on the capture's stream)");
+    }
+}
+
 enum { kNeedX = 1, kNeedW = 2, kNeedR = 4, kHasR = 8, kXIsBf16 = 16 };
 
 struct RMSNorm : torch::autograd::Function<RMSNorm> {
@@ -355,6 +372,7 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
     }
 
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        no_default_stream_behind_a_capture();
         const int64_t flags = ctx->saved_data["flags"].toInt();
         const auto saved = ctx->get_saved_variables();
         torch::autograd::variable_list out;
