@@ -1,7 +1,7 @@
 """Builds libodwscl.so (every HIP kernel + the C-ABI) for gfx950 and _bind.so (torch-side glue in front of it), in-tree.
 
 hipcc cross-compiles without a GPU, so this also runs in the CPU-only build
-container; the resulting .so is git-ignored but ships with gpurun snapshots.
+container; the resulting .so is git-ignored.
 """
 import glob
 import json
@@ -16,8 +16,8 @@ RECORD = os.path.join(HERE, "build", "commands.json")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 # -ffp-contract=off: ROI bin / sample coordinates must round exactly like the
-# reference's separate fp32 mul and add (SURVEY.md s7 hard part vii); kernels
-# that want FMAs ask for them explicitly (fmaf / MFMA).
+# reference's separate fp32 mul and add; kernels that want FMAs ask for them
+# explicitly (fmaf / MFMA).
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 -- the compiler forms them from ordinary float code, and some of their
 # forms have given wrong results on this hardware now and then (hipcc's host pass warns that it does not know the feature).
 FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",

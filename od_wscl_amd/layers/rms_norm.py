@@ -12,9 +12,9 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
 
     x (..., D) fp32 or bf16, any row pitch; weight (D,) fp32 or bf16 or None; residual of x's shape, in x's type or fp32 (h has its
     type; it is rounded once, and y is the norm of the rounded h).  Statistics and products are fp32, y is rounded once to x's type.
-    Gradients for x, weight and residual: the weight's summed over the rows in fp32, in one order; no second
-    and no forward-mode derivatives (refused).  h^2 has to fit fp32.  A backward pass can be captured into a HIP graph; where a graph made on
-    the default stream before still holds a node that it would reach, that is refused."""
+    Gradients for x, weight and residual: the weight's summed over the rows in fp32, in one order; no second and no forward-mode
+    derivatives (refused).  h^2 has to fit fp32.  A backward pass can be captured into a HIP graph; where a graph made on the default
+    stream before still holds a node that it would reach, that is refused."""
     return L.bind().rms_norm(x, weight, residual, eps)
 
 
